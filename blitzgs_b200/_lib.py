@@ -48,6 +48,14 @@ SIGNATURES = {
     "blitz_adam_update": (_i32, [_vp, _vp, _vp, _vp, _vp, _f32, _f32, _f32, _f32, _i64, _i64, _vp]),
     "blitz_adam_update_rows": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _f32, _f32, _f32, _f32, _f32, _i64, _i64,
                                       _vp]),
+    "blitz_quant_rows_write": (_i32, [_vp, _i32, _i64, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp,
+                                      _vp]),
+    "blitz_quant_rows_read": (_i32, [_vp, _vp, _i32, _vp, _i64, _i64, _i64, _i32, _vp, _i32, _vp]),
+    "blitz_adam8_update": (_i32, [_vp] * 8 + [_i64] + [_f32] * 7 + [_i64, _i64, _i32, _i32, _vp, _vp]),
+    "blitz_orthogonalize_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "blitz_orthogonalize": (_i32, [_vp, _i32, _vp, _i64, _i64, _i64, _i32, _f32, _f32, _f32, _f32, _vp, _sz, _vp]),
+    "blitz_orthogonal_update": (_i32, [_vp, _vp, _i32, _vp, _i64, _i64, _i64, _i32] + [_f32] * 6 + [_i32, _f32, _f32,
+                                                                                                    _vp, _sz, _vp]),
     "blitz_preprocess_backward_raw": (_i32, [
         _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _f32, _vp, _vp, _vp, _f32,
         _f32, _i32, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp,

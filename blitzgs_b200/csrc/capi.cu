@@ -1,4 +1,5 @@
 // extern "C" entry points (declared in include/blitzgs_b200.h).
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
@@ -7,6 +8,7 @@
 #include "blitzgs_b200.h"
 #include "common.cuh"
 #include "kernels.h"
+#include "ortho.h"
 
 using namespace blitz;
 
@@ -27,6 +29,95 @@ int fail(int code, const char* what) {
 int check(int code, const char* what) { return code == 0 ? 0 : fail(code, what); }
 
 inline cudaStream_t S(void* s) { return reinterpret_cast<cudaStream_t>(s); }
+
+// Whether the iterates stay inside what the kernels' scaled f16 terms hold:
+// singular values s in [0, 1] under s <- s (a + b s^2 + c s^4), largest values
+// of either polynomial at an end or where its derivative is zero.
+bool ortho_coefficients_ok(double a, double b, double c, int steps) {
+  if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return false;
+  double top = 1.0;
+  for (int k = 0; k < steps; ++k) {
+    const double t2 = top * top;
+    auto q = [&](double l) { return std::fabs(a + b * l + c * l * l); };
+    double most_q = std::fmax(q(0.0), q(t2)), most_p = top * q(t2);
+    if (c != 0.0) {
+      const double l = -b / (2.0 * c), root = 9.0 * b * b - 20.0 * a * c;
+      if (l > 0.0 && l < t2) most_q = std::fmax(most_q, q(l));
+      if (root >= 0.0)
+        for (int sign = -1; sign <= 1; sign += 2) {
+          const double z = (-3.0 * b + sign * std::sqrt(root)) / (10.0 * c);
+          if (z > 0.0 && z < t2) most_p = std::fmax(most_p, std::sqrt(z) * q(z));
+        }
+    } else if (b != 0.0) {
+      const double z = -a / (3.0 * b);
+      if (z > 0.0 && z < t2) most_p = std::fmax(most_p, std::sqrt(z) * q(z));
+    }
+    if (most_q > 7.8 || most_p > 1.85) return false;
+    top = std::fmax(most_p, 1e-30);
+  }
+  return true;
+}
+
+// the fields orthogonalisation's two entries share; 0 or an error code
+int ortho_fields(OrthoParams& p, const char* name, int type, int64_t batch, int64_t rows, int64_t cols, int steps,
+                 float a, float b, float c, float eps) {
+  const int64_t most = 32768;
+  char text[160];
+  snprintf(text, sizeof(text), "%s: bad sizes, type or steps", name);
+  if (batch < 0 || rows < 0 || cols < 0 || rows > most || cols > most || type < 0 || type > 2 || steps < 1 ||
+      steps > 64 || !(eps >= 0.0f))
+    return fail(BLITZ_EINVAL, text);
+  if (rows > 0 && cols > 0 && batch > ((int64_t)1 << 38) / (((rows + 127) / 128 * 128) * ((cols + 127) / 128 * 128)))
+    return fail(BLITZ_EINVAL, text);
+  if (!ortho_coefficients_ok(a, b, c, steps)) {
+    snprintf(text, sizeof(text), "%s: coefficients let the iterates grow beyond 1.85 or the polynomial beyond 7.8", name);
+    return fail(BLITZ_EINVAL, text);
+  }
+  p.g_type = type;
+  p.batch = batch;
+  const bool tall = rows > cols;
+  p.n = tall ? cols : rows;
+  p.m = tall ? rows : cols;
+  p.si = tall ? 1 : cols;
+  p.sj = tall ? cols : 1;
+  p.steps = steps;
+  p.a = a;
+  p.b = b;
+  p.c = c;
+  p.eps = eps;
+  return 0;
+}
+
+int ortho_start(const OrthoParams& p, const char* name, void* workspace, size_t workspace_bytes, void* stream) {
+  const size_t need = ortho_workspace_bytes(p);
+  char text[160];
+  snprintf(text, sizeof(text), "%s: workspace smaller than *_workspace_bytes or not 256-byte aligned", name);
+  if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u)))
+    return fail(BLITZ_ESCRATCH, text);
+  return check(launch_ortho(p, workspace, S(stream)), name);
+}
+
+// 32 lanes a (row, group) at most, 256 threads a block, 2^31 - 1 blocks
+inline bool too_many_units(int64_t n, int64_t D, int group) {
+  const int64_t G = (D + group - 1) / group, most = ((int64_t)1 << 31) * 8 - 8;
+  return G > 0 && n > most / G;
+}
+
+// the checks and fields that the row store's write and read share
+int quant_sizes(QuantParams& q, int kind, const int64_t* rows, int64_t n, int64_t N, int64_t D, int group,
+                const char* what) {
+  if (n < 0 || N < 0 || D < 0 || D > ((int64_t)1 << 30) || group < 1 || group > 256 || kind < 0 || kind > 1 ||
+      q.type < 0 || q.type > 2 || (!rows && n > N) || too_many_units(n, D, group))
+    return fail(BLITZ_EINVAL, what);
+  q.kind = kind;
+  q.rows = rows;
+  q.n = n;
+  q.N = N;
+  q.D = D;
+  q.group = group;
+  q.G = (int)((D + group - 1) / group);
+  return 0;
+}
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -589,6 +680,115 @@ int blitz_adam_update_rows(float* param, const float* grad_rows, float* exp_avg,
   a.N = N;
   a.M = M;
   return check(launch_adam(a, S(stream)), "blitz_adam_update_rows");
+}
+
+int blitz_quant_rows_write(const void* values, int value_type, int64_t value_stride, void* codes, float* scales,
+                           int kind, const int64_t* rows, int64_t n, int64_t N, int64_t D, int group, int dither,
+                           uint32_t seed, const int64_t* seed_ptr, void* stream) {
+  QuantParams q{};
+  q.values = values;
+  q.value_stride = value_stride;
+  q.type = value_type;
+  q.codes = static_cast<uint8_t*>(codes);
+  q.scales = scales;
+  q.dither = dither != 0;
+  q.seed = seed;
+  q.seed_ptr = seed_ptr;
+  if (int rc = quant_sizes(q, kind, rows, n, N, D, group, "blitz_quant_rows_write: bad sizes, type or kind")) return rc;
+  if (value_stride < D) return fail(BLITZ_EINVAL, "blitz_quant_rows_write: value_stride smaller than D");
+  if (n == 0 || D == 0) return 0;
+  if (!values || !codes || !scales) return fail(BLITZ_EINVAL, "blitz_quant_rows_write: null pointer");
+  return check(launch_quant_write(q, S(stream)), "blitz_quant_rows_write");
+}
+
+int blitz_quant_rows_read(const void* codes, const float* scales, int kind, const int64_t* rows, int64_t n, int64_t N,
+                          int64_t D, int group, void* out, int value_type, void* stream) {
+  QuantParams q{};
+  q.out = out;
+  q.type = value_type;
+  q.codes = const_cast<uint8_t*>(static_cast<const uint8_t*>(codes));
+  q.scales = const_cast<float*>(scales);
+  if (int rc = quant_sizes(q, kind, rows, n, N, D, group, "blitz_quant_rows_read: bad sizes, type or kind")) return rc;
+  if (n == 0 || D == 0) return 0;
+  if (!out || (N > 0 && (!codes || !scales))) return fail(BLITZ_EINVAL, "blitz_quant_rows_read: null pointer");
+  return check(launch_quant_read(q, S(stream)), "blitz_quant_rows_read");
+}
+
+int blitz_adam8_update(float* param, const float* grad, void* m_codes, float* m_scales, void* r_codes,
+                       float* r_scales, const uint8_t* visible, const int64_t* rows, int64_t n_rows, float grad_scale,
+                       float lr, float b1, float one_minus_b1, float b2, float one_minus_b2, float eps, int64_t N,
+                       int64_t M, int group, uint32_t seed, const int64_t* seed_ptr, void* stream) {
+  if (N < 0 || M <= 0 || n_rows < 0 || group < 1 || group > 256 || too_many_units(rows ? n_rows : N, M, group))
+    return fail(BLITZ_EINVAL, "blitz_adam8_update: bad sizes");
+  if ((visible != nullptr) == (rows != nullptr) && (rows || N > 0))
+    return fail(BLITZ_EINVAL, "blitz_adam8_update: give either visible or rows");
+  Adam8Params a{};
+  a.n = rows ? n_rows : N;
+  if (a.n == 0) return 0;
+  if (!param || !grad || !m_codes || !m_scales || !r_codes || !r_scales)
+    return fail(BLITZ_EINVAL, "blitz_adam8_update: null pointer");
+  a.param = param;
+  a.grad = grad;
+  a.m_codes = static_cast<uint8_t*>(m_codes);
+  a.r_codes = static_cast<uint8_t*>(r_codes);
+  a.m_scales = m_scales;
+  a.r_scales = r_scales;
+  a.visible = reinterpret_cast<const bool*>(visible);
+  a.rows = rows;
+  a.N = N;
+  a.M = M;
+  a.group = group;
+  a.G = (int)((M + group - 1) / group);
+  a.lr = lr;
+  a.b1 = b1;
+  a.b1c = one_minus_b1;
+  a.b2 = b2;
+  a.b2c = one_minus_b2;
+  a.eps = eps;
+  a.grad_scale = grad_scale;
+  a.seed = seed;
+  a.seed_ptr = seed_ptr;
+  return check(launch_adam8(a, S(stream)), "blitz_adam8_update");
+}
+
+size_t blitz_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols) {
+  OrthoParams p{};
+  if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
+  p.batch = batch;
+  p.n = rows < cols ? rows : cols;
+  p.m = rows < cols ? cols : rows;
+  return ortho_workspace_bytes(p);
+}
+
+int blitz_orthogonalize(const void* g, int value_type, void* out, int64_t batch, int64_t rows, int64_t cols, int steps,
+                        float a, float b, float c, float eps, void* workspace, size_t workspace_bytes, void* stream) {
+  OrthoParams p{};
+  if (int rc = ortho_fields(p, "blitz_orthogonalize", value_type, batch, rows, cols, steps, a, b, c, eps)) return rc;
+  if (batch == 0 || rows == 0 || cols == 0) return 0;
+  if (!g || !out) return fail(BLITZ_EINVAL, "blitz_orthogonalize: null pointer");
+  p.g = g;
+  p.out = out;
+  return ortho_start(p, "blitz_orthogonalize", workspace, workspace_bytes, stream);
+}
+
+int blitz_orthogonal_update(float* param, const void* grad, int value_type, float* momentum, int64_t batch,
+                            int64_t rows, int64_t cols, int steps, float a, float b, float c, float eps, float beta,
+                            float one_minus_beta, int nesterov, float keep, float alpha, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  OrthoParams p{};
+  if (int rc = ortho_fields(p, "blitz_orthogonal_update", value_type, batch, rows, cols, steps, a, b, c, eps))
+    return rc;
+  if (batch == 0 || rows == 0 || cols == 0) return 0;
+  if (!param || !grad || !momentum) return fail(BLITZ_EINVAL, "blitz_orthogonal_update: null pointer");
+  p.param = param;
+  p.g = grad;
+  p.momentum = momentum;
+  p.beta = beta;
+  p.one_minus_beta = one_minus_beta;
+  p.nesterov = nesterov;
+  p.keep = keep;
+  p.alpha = alpha;
+  return ortho_start(p, "blitz_orthogonal_update", workspace, workspace_bytes, stream);
 }
 
 size_t blitz_exchange_pack_scratch_bytes(int64_t n_rows, int n_ranks) {

@@ -282,6 +282,43 @@ struct AdamParams {
 };
 int launch_adam(const AdamParams& p, cudaStream_t st);
 
+// Rows held in 8 bits (see quant_rows.cu).  rows == null: all N rows in order.
+enum : int { kValueF32 = 0, kValueBf16 = 1, kValueF16 = 2 };
+struct QuantParams {
+  const void* values;    // write: [n] rows of D values, value_stride apart
+  int64_t value_stride;
+  void* out;             // read: [n, D]
+  int type;              // of values / out
+  int kind;              // quant::Kind
+  uint8_t* codes;        // [N, D]
+  float* scales;         // [N, G]
+  const int64_t* rows;   // [n] or null
+  int64_t n, N, D;
+  int group, G;
+  bool dither;
+  uint32_t seed;
+  const int64_t* seed_ptr;  // device, added to seed, or null
+};
+int launch_quant_write(const QuantParams& p, cudaStream_t st);
+int launch_quant_read(const QuantParams& p, cudaStream_t st);
+
+// Sparse Adam on moments held in 8 bits.  rows given: grad is [n, M] for
+// Gaussians rows[j]; else n == N, grad is [N, M] and visible [N] is given.
+struct Adam8Params {
+  float* param;
+  const float* grad;
+  uint8_t *m_codes, *r_codes;   // [N, M]
+  float *m_scales, *r_scales;   // [N, G]
+  const bool* visible;
+  const int64_t* rows;
+  int64_t n, N, M;
+  int group, G;
+  float lr, b1, b1c, b2, b2c, eps, grad_scale;  // b1c = 1 - b1, b2c = 1 - b2
+  uint32_t seed;
+  const int64_t* seed_ptr;
+};
+int launch_adam8(const Adam8Params& p, cudaStream_t st);
+
 // Pack rows [0, n_rows) of a camera's exchange records into the send buffer:
 // row j goes to every rank r whose bit is set in mask[j], at
 // dest_offset[r] + (its running position among rank r's rows); send_row

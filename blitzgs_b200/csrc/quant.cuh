@@ -1,0 +1,118 @@
+// Rows of values held in 8 bits: per group of consecutive values one float
+// scale s, and per value a code q with value = q * s.
+//   int8: s = max|x| / 127, q in [-127, 127] (s a step less where 127 s would
+//         pass the largest float);
+//   e4m3: s = the smallest power of two (at least 2^-126) with max|x| / s <= 448,
+//         so that x / s and q * s are exact and storing stored values again
+//         changes nothing.  The format's own exponent covers 2^-9 .. 448 (.. 240
+//         with s = 2^120, so that every stored value is finite).
+// A group of zeros has s = 0; a group that holds a NaN or an infinity has
+// s = NaN and reads back as NaN throughout: nothing non-finite is hidden.
+// q is x / s rounded to nearest even or, dithered, floor(|x / s| / step + u)
+// steps with u in [0, 1) from a hash of (seed, row, column): the expected
+// value of a stored number is then the number, which a moving average whose
+// change per step is below half a step needs (rounded to nearest, it stands).
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <cfloat>
+#include <cstdint>
+
+namespace blitz {
+namespace quant {
+
+enum Kind : int { kInt8 = 0, kE4m3 = 1 };
+
+__device__ __forceinline__ uint32_t row_key(uint32_t seed, int64_t row) {
+  uint32_t k = seed * 0x9E3779B1u + (uint32_t)row * 0x85EBCA77u;
+  k = (k ^ (k >> 16)) * 0x7FEB352Du;
+  k = (k ^ (k >> 15)) * 0x846CA68Bu;
+  return k ^ (k >> 16);
+}
+
+// 20 random bits in [0, 1): x / step has at most 20 bits below one where the
+// format is normal, so the sum before the floor is exact there
+__device__ __forceinline__ float uniform20(uint32_t key, uint32_t col) {
+  uint32_t h = key + col * 0x9E3779B1u;
+  h = (h ^ (h >> 15)) * 0x2C1B3C6Du;
+  h = h ^ (h >> 12);
+  return (float)(h >> 12) * 0x1p-20f;
+}
+
+// the group's scale, and what x is multiplied by (e4m3) before it is rounded
+template <int KIND>
+__device__ __forceinline__ float group_scale(float amax, bool finite) {
+  if (!finite) return __int_as_float(0x7fffffff);
+  if (KIND == kInt8) {
+    const float s = __fdiv_rn(amax, 127.0f);
+    // next to the largest float 127 s may round to infinity: one step less
+    return __fmul_rn(s, 127.0f) <= FLT_MAX ? s : __int_as_float(__float_as_int(s) - 1);
+  }
+  const int bits = __float_as_int(amax);
+  // amax = 1.f * 2^e: 448 = 1.75 * 2^8, so s = 2^(e-8) while 1.f <= 1.75
+  const int e = max((bits >> 23) - 8 + ((bits & 0x7fffff) > 0x600000 ? 1 : 0), 1);
+  return amax > 0.0f ? __int_as_float(e << 23) : 0.0f;
+}
+
+// 1 / s of a power of two s >= 2^-126 (s <= 2^120 for any finite group); 0 for 0
+__device__ __forceinline__ float inverse_pow2(float s) {
+  return s > 0.0f ? __int_as_float((254 << 23) - __float_as_int(s)) : 0.0f;
+}
+
+// x -> code.  s: the group's scale; inv: inverse_pow2(s) (e4m3 only).
+template <int KIND, bool DITHER, bool NEVER_ZERO = false>
+__device__ __forceinline__ uint8_t encode(float x, float s, float inv, float u) {
+  if (KIND == kInt8) {
+    // a true division, so that the rounding is of x / s itself
+    const float y = s > 0.0f ? __fdiv_rn(x, s) : 0.0f;
+    const float q = DITHER ? floorf(__fadd_rn(y, u)) : rintf(y);
+    return (uint8_t)(int8_t)(int)fminf(fmaxf(q, -127.0f), 127.0f);
+  } else {
+    float y = __fmul_rn(x, inv);
+    if (DITHER) {
+      const float mag = fabsf(y);
+      // step = 2^(floor(log2 mag) - 3), 2^-9 below the normal numbers
+      const int b = max(__float_as_int(mag) & 0x7f800000, 121 << 23);
+      const float inv_step = __int_as_float((254 << 23) + (3 << 23) - b);
+      const float q = floorf(__fadd_rn(__fmul_rn(mag, inv_step), u));
+      y = copysignf(__fmul_rn(q, __int_as_float(b - (3 << 23))), y);
+    }
+    // where x > 0, the smallest code at least (x is never negative there)
+    if (NEVER_ZERO) y = x > 0.0f ? fmaxf(y, 0x1p-9f) : y;
+    // 256 * 2^120 is past the largest float: 240 is the code below it
+    if (s >= 0x1p120f) y = fminf(fmaxf(y, -240.0f), 240.0f);
+    return (uint8_t)__nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+  }
+}
+
+template <int KIND>
+__device__ __forceinline__ float decode(uint8_t c, float s) {
+  if (KIND == kInt8) return __fmul_rn((float)(int8_t)c, s);
+  const __half_raw h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)c, __NV_E4M3);
+  return __fmul_rn(__half2float(__half(h)), s);
+}
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+template <class T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+
+// maximum over LANES neighbouring lanes (a power of two)
+template <int LANES>
+__device__ __forceinline__ float lanes_max(float v) {
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+}  // namespace quant
+}  // namespace blitz

@@ -938,3 +938,206 @@ def adam_update_rows(param, grad_rows, exp_avg, exp_avg_sq, rows, lr, b1, b2, ep
     _lib.call("blitz_adam_update_rows", ptr(param), ptr(grad_rows), ptr(exp_avg), ptr(exp_avg_sq), ptr(rows), n,
               float(grad_scale), float(lr), float(b1), float(b2), float(eps), int(N), int(M), _lib.stream_ptr())
     TIMER.end(tok, N=int(N), M=int(M), n_rows=n)
+
+
+_VALUE_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_CODE_KINDS = {torch.int8: 0, torch.float8_e4m3fn: 1}
+
+
+def _same_device(first, *others):
+    """All tensors on one GPU, the current device: the launch goes to the
+    current device's current stream."""
+    _require_cuda(first, *others)
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise RuntimeError(f"tensors on different devices: {first.device} and {t.device}")
+    if first.device.index != torch.cuda.current_device():
+        raise RuntimeError(f"tensors on {first.device}, but the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _code_rows(codes, scales, group, what):
+    """(N, D) of a store's contiguous codes [N, D] (int8 or float8_e4m3fn) and
+    scales [N, ceil(D / group)]."""
+    if codes.dtype not in _CODE_KINDS:
+        raise RuntimeError(f"{what}: codes are int8 or float8_e4m3fn, got {codes.dtype}")
+    if scales.dtype != torch.float32 or not codes.is_contiguous() or not scales.is_contiguous():
+        raise RuntimeError(f"{what} needs contiguous codes and contiguous float32 scales")
+    if not 1 <= group <= 256:
+        raise RuntimeError(f"{what}: a group holds 1 to 256 values, got {group}")
+    if codes.dim() != 2 or tuple(scales.shape) != (codes.shape[0], -(-codes.shape[1] // group)):
+        raise RuntimeError(f"{what}: codes {tuple(codes.shape)} in groups of {group} need scales "
+                           f"[{codes.shape[0]}, ceil(D / group)], got {tuple(scales.shape)}")
+    return codes.shape
+
+
+def _row_list(rows, device, what):
+    if rows.dim() != 1 or rows.dtype not in (torch.int64, torch.int32):
+        raise RuntimeError(f"{what}: rows is a one-dimensional int64 or int32 tensor")
+    return rows.to(torch.int64).contiguous()
+
+
+def _seed(seed, device):
+    """A seed as (32-bit integer, device tensor or None): an int64 tensor of
+    one element is read by the kernel, so a captured step can count it up."""
+    if isinstance(seed, torch.Tensor):
+        if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != device:
+            raise RuntimeError("a seed tensor is one int64 on the same GPU")
+        return 0, seed
+    return int(seed) & 0xFFFFFFFF, None
+
+
+def quant_rows_write(values, codes, scales, rows=None, *, group, seed=None):
+    """Store values [n, D] (float32, bfloat16 or float16) at the rows (int64
+    [n], distinct; None: all rows in order) of an 8-bit store: codes [N, D]
+    (int8, or float8_e4m3fn with power-of-two scales) and float32 scales
+    [N, ceil(D / group)] (blitz_quant_rows_write).  Rows outside [0, N) are
+    skipped.  ``seed`` (an int or an int64 tensor of one element) dithers the
+    rounding; None rounds to nearest even."""
+    _same_device(values, codes, scales, rows)
+    N, D = _code_rows(codes, scales, group, "quant_rows_write")
+    n = N if rows is None else rows.numel()
+    if values.dtype not in _VALUE_TYPES or tuple(values.shape) != (n, D):
+        raise RuntimeError(f"quant_rows_write: values of 32 or 16 bits [{n}, {D}] wanted, got {values.dtype} "
+                           f"{tuple(values.shape)}")
+    if rows is not None:
+        rows = _row_list(rows, codes.device, "quant_rows_write")
+    if D > 1 and values.stride(1) != 1 or n > 1 and values.stride(0) < D:
+        values = values.contiguous()
+    s, s_ptr = (0, None) if seed is None else _seed(seed, codes.device)
+    tok = TIMER.begin("quant_write")
+    _lib.call("blitz_quant_rows_write", ptr(values), _VALUE_TYPES[values.dtype], values.stride(0) if n > 1 else D,
+              ptr(codes), ptr(scales), _CODE_KINDS[codes.dtype], ptr(rows), n, N, D, int(group),
+              int(seed is not None), s, ptr(s_ptr), _lib.stream_ptr())
+    TIMER.end(tok, n_rows=n, D=D)
+
+
+def quant_rows_read(codes, scales, rows=None, *, group, dtype=torch.float32):
+    """The rows (int64 [n]; None: all) of an 8-bit store as values [n, D] in
+    dtype (blitz_quant_rows_read); rows outside [0, N) read as zeros."""
+    _same_device(codes, scales, rows)
+    N, D = _code_rows(codes, scales, group, "quant_rows_read")
+    if dtype not in _VALUE_TYPES:
+        raise RuntimeError(f"quant_rows_read: values are of 32 or 16 bits, got {dtype}")
+    if rows is not None:
+        rows = _row_list(rows, codes.device, "quant_rows_read")
+    n = N if rows is None else rows.numel()
+    out = torch.empty((n, D), dtype=dtype, device=codes.device)
+    tok = TIMER.begin("quant_read")
+    _lib.call("blitz_quant_rows_read", ptr(codes), ptr(scales), _CODE_KINDS[codes.dtype], ptr(rows), n, N, D,
+              int(group), ptr(out), _VALUE_TYPES[dtype], _lib.stream_ptr())
+    TIMER.end(tok, n_rows=n, D=D)
+    return out
+
+
+def _adam8(param, grad, m_codes, m_scales, r_codes, r_scales, visible, rows, n, lr, b1, b2, eps, N, M, group, seed,
+           grad_scale, what):
+    _same_device(param, grad, m_codes, m_scales, r_codes, r_scales, visible, rows)
+    if param.dtype != torch.float32 or not param.is_contiguous() or param.numel() != N * M:
+        raise RuntimeError(f"{what} needs a contiguous float32 parameter of N * M values")
+    if grad.dtype != torch.float32 or grad.numel() != n * M:
+        raise RuntimeError(f"{what} needs a float32 gradient of {n} rows of {M} values")
+    for c, s in ((m_codes, m_scales), (r_codes, r_scales)):
+        if tuple(_code_rows(c, s, group, what)) != (N, M) or c.dtype != torch.float8_e4m3fn:
+            raise RuntimeError(f"{what} needs float8_e4m3fn moments [{N}, {M}]")
+    grad = grad.contiguous()
+    s, s_ptr = _seed(seed, param.device)
+    tok = TIMER.begin("adam8")
+    _lib.call("blitz_adam8_update", ptr(param), ptr(grad), ptr(m_codes), ptr(m_scales), ptr(r_codes), ptr(r_scales),
+              ptr(visible), ptr(rows), n, float(grad_scale), float(lr), float(b1), 1.0 - float(b1), float(b2),
+              1.0 - float(b2), float(eps), N, M, int(group), s, ptr(s_ptr), _lib.stream_ptr())
+    TIMER.end(tok, N=N, M=M, n_rows=n)
+
+
+def adam8_update(param, grad, m_codes, m_scales, r_codes, r_scales, visible, lr, b1, b2, eps, N, M, *, group, seed,
+                 grad_scale=1.0):
+    """In-place sparse Adam step of param [N*M] for the Gaussians with
+    visible[g], its first moment and the root of its second kept in 8-bit
+    stores (float8_e4m3fn codes [N, M], float32 scales [N, ceil(M / group)];
+    blitz_adam8_update).  ``seed``: of the dithered rounding of the new
+    moments, another one each step (an int, or an int64 tensor of one element)."""
+    if visible.numel() != N:
+        raise RuntimeError(f"adam8_update: visible has {visible.numel()} entries for {N} Gaussians")
+    visible = visible.to(torch.bool).contiguous()
+    _adam8(param, grad, m_codes, m_scales, r_codes, r_scales, visible, None, N, lr, b1, b2, eps, N, M, group, seed,
+           grad_scale, "adam8_update")
+
+
+def adam8_update_rows(param, grad_rows, m_codes, m_scales, r_codes, r_scales, rows, lr, b1, b2, eps, N, M, *, group,
+                      seed, grad_scale=1.0):
+    """The same step for the Gaussians rows (int64 [n], distinct) whose
+    gradients are the rows of grad_rows [n, M]; rows outside [0, N) are skipped."""
+    rows = _row_list(rows, param.device, "adam8_update_rows")
+    _adam8(param, grad_rows, m_codes, m_scales, r_codes, r_scales, None, rows, rows.numel(), lr, b1, b2, eps, N, M,
+           group, seed, grad_scale, "adam8_update_rows")
+
+
+ORTHO_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def _matrices(t, what):
+    """(batch, rows, cols) of a tensor [..., rows, cols]."""
+    if t.dim() < 2:
+        raise RuntimeError(f"{what}: a matrix [..., rows, cols] wanted, got {tuple(t.shape)}")
+    rows, cols = t.shape[-2], t.shape[-1]
+    return t.numel() // (rows * cols) if rows and cols else 0, rows, cols
+
+
+def _ortho_workspace(batch, rows, cols, device):
+    """Device scratch of one call: from the caching allocator, so it belongs
+    to the call's stream, or to the graph it is captured into."""
+    need = _lib.load().blitz_orthogonalize_workspace_bytes(batch, rows, cols)
+    return (torch.empty(need, dtype=torch.uint8, device=device) if need else None), need
+
+
+def orthogonalize(g, *, steps=5, coefficients=ORTHO_COEFFICIENTS, eps=1e-7):
+    """The direction of each matrix of g [..., rows, cols] (float32, bfloat16
+    or float16): its singular values driven towards 1 by ``steps`` Newton-Schulz
+    steps (blitz_orthogonalize).  Returns a new tensor of g's type.  float32
+    and float16 results are within about 1e-5 (2-norm) of the formula before
+    their rounding, bfloat16 ones within about 2e-3."""
+    _same_device(g)
+    if g.dtype not in _VALUE_TYPES:
+        raise RuntimeError(f"orthogonalize: values are of 32 or 16 bits, got {g.dtype}")
+    batch, rows, cols = _matrices(g, "orthogonalize")
+    g = g.contiguous()
+    out = torch.empty_like(g)
+    ws, need = _ortho_workspace(batch, rows, cols, g.device)
+    a, b, c = coefficients
+    tok = TIMER.begin("orthogonalize")
+    _lib.call("blitz_orthogonalize", ptr(g), _VALUE_TYPES[g.dtype], ptr(out), batch, rows, cols, int(steps), a, b, c,
+              float(eps), ptr(ws), need, _lib.stream_ptr())
+    TIMER.end(tok, batch=batch, rows=rows, cols=cols)
+    return out
+
+
+def orthogonal_update(param, grad, momentum, lr, *, beta=0.95, nesterov=True, weight_decay=0.0, scale=None, steps=5,
+                      coefficients=ORTHO_COEFFICIENTS, eps=1e-7):
+    """One in-place step of a matrix parameter [..., rows, cols] along its
+    orthogonalised momentum (blitz_orthogonal_update):
+
+        momentum = beta momentum + (1 - beta) grad
+        u = (1 - beta) grad + beta momentum  (nesterov), else momentum
+        param = param (1 - lr weight_decay) - lr scale orthogonalize(u)
+
+    param and momentum are contiguous float32, grad float32, bfloat16 or
+    float16; scale defaults to sqrt(max(1, rows / cols))."""
+    _same_device(param, grad, momentum)
+    for t in (param, momentum):
+        if t.dtype != torch.float32 or not t.is_contiguous() or t.shape != param.shape:
+            raise RuntimeError("orthogonal_update needs contiguous float32 param and momentum of one shape")
+    if grad.dtype not in _VALUE_TYPES or grad.shape != param.shape:
+        raise RuntimeError("orthogonal_update needs a gradient of the parameter's shape, of 32 or 16 bits")
+    batch, rows, cols = _matrices(param, "orthogonal_update")
+    if batch and (param.data_ptr() == momentum.data_ptr() or grad.data_ptr() in (param.data_ptr(),
+                                                                                 momentum.data_ptr())):
+        raise RuntimeError("orthogonal_update needs param, grad and momentum in different memory")
+    grad = grad.contiguous()
+    if scale is None:
+        scale = math.sqrt(max(1.0, rows / cols)) if cols else 1.0
+    ws, need = _ortho_workspace(batch, rows, cols, param.device)
+    a, b, c = coefficients
+    tok = TIMER.begin("orthogonal_update")
+    _lib.call("blitz_orthogonal_update", ptr(param), ptr(grad), _VALUE_TYPES[grad.dtype], ptr(momentum), batch, rows,
+              cols, int(steps), a, b, c, float(eps), float(beta), 1.0 - float(beta), int(bool(nesterov)),
+              1.0 - float(lr) * float(weight_decay), float(lr) * float(scale), ptr(ws), need, _lib.stream_ptr())
+    TIMER.end(tok, batch=batch, rows=rows, cols=cols)

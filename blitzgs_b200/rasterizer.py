@@ -364,27 +364,29 @@ class SparseGaussianAdam(torch.optim.Adam):
             param = group["params"][0]
             if param.grad is None or param.grad.numel() == 0:
                 continue
-            state = self.state[param]
-            if len(state) == 0:
-                state["step"] = torch.tensor(0.0, dtype=torch.float32)
-                state["exp_avg"] = torch.zeros_like(param, memory_format=torch.preserve_format)
-                state["exp_avg_sq"] = torch.zeros_like(param, memory_format=torch.preserve_format)
-            exp_avg, exp_avg_sq = state["exp_avg"], state["exp_avg_sq"]
-            state["step"] += 1
-            step = state["step"]
-            lr_t = lr * (1 - 0.999 ** step) ** 0.5 / (1 - 0.9 ** step)
-            n = N if N is not None else param.shape[0]
-            M = param.numel() // n
-            g = param.grad
-            if g.is_sparse:
-                g = g.coalesce()
-                rows = g.indices()[0]
-                ops.adam_update_rows(param, g.values().reshape(rows.numel(), M), exp_avg, exp_avg_sq, rows,
-                                     float(lr_t), 0.9, 0.999, eps, n, M, grad_scale=1.0 if scale is None else scale)
-            else:
-                if scale is not None:
-                    g = g * scale
-                _C.adamUpdate(param, g, exp_avg, exp_avg_sq, visibility, float(lr_t), 0.9, 0.999, eps, n, M)
+            self._update(param, self.state[param], N if N is not None else param.shape[0], visibility, lr, eps, scale)
+
+    def _update(self, param, state, n, visibility, lr, eps, scale):
+        """The step of one group's parameter, n rows; scale (or None) multiplies the gradient first."""
+        if len(state) == 0:
+            state["step"] = torch.tensor(0.0, dtype=torch.float32)
+            state["exp_avg"] = torch.zeros_like(param, memory_format=torch.preserve_format)
+            state["exp_avg_sq"] = torch.zeros_like(param, memory_format=torch.preserve_format)
+        exp_avg, exp_avg_sq = state["exp_avg"], state["exp_avg_sq"]
+        state["step"] += 1
+        step = state["step"]
+        lr_t = lr * (1 - 0.999 ** step) ** 0.5 / (1 - 0.9 ** step)
+        M = param.numel() // n
+        g = param.grad
+        if g.is_sparse:
+            g = g.coalesce()
+            rows = g.indices()[0]
+            ops.adam_update_rows(param, g.values().reshape(rows.numel(), M), exp_avg, exp_avg_sq, rows,
+                                 float(lr_t), 0.9, 0.999, eps, n, M, grad_scale=1.0 if scale is None else scale)
+        else:
+            if scale is not None:
+                g = g * scale
+            _C.adamUpdate(param, g, exp_avg, exp_avg_sq, visibility, float(lr_t), 0.9, 0.999, eps, n, M)
 
 
 # ---------------------------------------------------------------------------

@@ -33,6 +33,10 @@ import torch.distributed as dist
 
 from .distributed import _spread_bits
 
+# the optimizer state that has one row per Gaussian: SparseGaussianAdam's
+# moments, or the 8-bit codes and scales of SparseGaussianAdam8bit
+MOMENTS = ("exp_avg", "exp_avg_sq", "exp_avg_codes", "exp_avg_scales", "exp_root_codes", "exp_root_scales")
+
 
 def _counts(n_local, group, device):
     ws = dist.get_world_size(group)
@@ -147,8 +151,8 @@ def redistribute(params, optimizer=None, group=None, mode="zorder", threshold=1.
     the first being the positions [n, 3] (the reference's order: xyz,
     features_dc, features_rest, opacity, scaling, rotation).  ``optimizer``
     (one parameter per group, as the reference's Adam and
-    SparseGaussianAdam): its exp_avg / exp_avg_sq travel with their rows and
-    its groups are rebuilt around the new parameters.  ``densify`` (a
+    SparseGaussianAdam, or SparseGaussianAdam8bit): its moments travel with
+    their rows and its groups are rebuilt around the new parameters.  ``densify`` (a
     densify.DensificationStats) is re-created for the new shard size, zeroed
     as the reference resets its statistics.
 
@@ -171,10 +175,10 @@ def redistribute(params, optimizer=None, group=None, mode="zorder", threshold=1.
     if optimizer is not None:
         for p in params:
             st = optimizer.state.get(p, {})
-            states.append([k for k in ("exp_avg", "exp_avg_sq") if k in st])
+            states.append([k for k in MOMENTS if k in st])
         # every rank must move the same moments, or the exchanges below pair
         # different tensors (or wait for ever): agree first, fail together
-        have = torch.tensor([[k in keys for k in ("exp_avg", "exp_avg_sq")] for keys in states],
+        have = torch.tensor([[k in keys for k in MOMENTS] for keys in states],
                             dtype=torch.int32, device=dev).reshape(-1)
         lo_have, hi_have = have.clone(), have.clone()
         dist.all_reduce(lo_have, op=dist.ReduceOp.MIN, group=group)

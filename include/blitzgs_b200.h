@@ -524,6 +524,77 @@ int blitz_adam_update_rows(float* param, const float* grad_rows, float* exp_avg,
                            float eps, int64_t N, int64_t M, void* stream);
 
 /*
+ * Rows of values held in 8 bits (no reference counterpart: the reference
+ * keeps every optimizer state in 32 bits).  codes [N, D] and scales [N, G],
+ * G = ceil(D / group), group 1..256: value = code * scale of its group.
+ *   kind 0, int8: scale = max|x| / 127, code = x / scale rounded;
+ *   kind 1, e4m3: scale = the smallest power of two (>= 2^-126) with
+ *     max|x| / scale <= 448 (0 for a group of zeros), code = x / scale rounded
+ *     to e4m3; storing values read from such a store changes nothing.
+ * A group with a NaN or an infinity gets a NaN scale and reads back as NaN.
+ * value_type: 0 float, 1 bf16, 2 fp16.
+ *
+ * write stores values (row j value_stride elements after row j - 1) at row
+ * rows[j] (int64, distinct; null: row j); rows outside [0, N) are skipped and
+ * rows not listed keep their bytes.  dither 0 rounds to nearest even;
+ * dither 1 rounds down after adding u steps, u = 20 bits of a hash of
+ * (seed, row, column), seed = seed + *seed_ptr (device, may be null; one that
+ * a captured graph's step counts up gives each replay its own).
+ * read decodes row rows[j] (null: row j) into row j of out [n, D]; a row
+ * outside [0, N) becomes zeros.
+ */
+int blitz_quant_rows_write(const void* values, int value_type, int64_t value_stride, void* codes, float* scales,
+                           int kind, const int64_t* rows, int64_t n, int64_t N, int64_t D, int group, int dither,
+                           uint32_t seed, const int64_t* seed_ptr, void* stream);
+int blitz_quant_rows_read(const void* codes, const float* scales, int kind, const int64_t* rows, int64_t n, int64_t N,
+                          int64_t D, int group, void* out, int value_type, void* stream);
+
+/*
+ * The sparse Adam step on moments held in such rows (kind e4m3): m_codes /
+ * m_scales hold the first moment, r_codes / r_scales the ROOT of the second.
+ * For every element of an updated Gaussian, with g = grad * grad_scale,
+ *   m = b1 m + one_minus_b1 g;  r = sqrt(b2 r^2 + one_minus_b2 g^2);
+ *   param -= lr m / (r + eps)
+ * in 32 bits, and then m and r are stored again, dithered as by
+ * blitz_quant_rows_write (r with seed ^ 0x5BF03635, and never to zero where
+ * it is positive).  Give either visible (uint8 [N], grad [N, M]) or
+ * rows (int64 [n_rows], distinct, grad [n_rows, M]); rows outside [0, N) are
+ * skipped, and the other Gaussians keep their parameter and state.
+ */
+int blitz_adam8_update(float* param, const float* grad, void* m_codes, float* m_scales, void* r_codes,
+                       float* r_scales, const uint8_t* visible, const int64_t* rows, int64_t n_rows, float grad_scale,
+                       float lr, float b1, float one_minus_b1, float b2, float one_minus_b2, float eps, int64_t N,
+                       int64_t M, int group, uint32_t seed, const int64_t* seed_ptr, void* stream);
+
+/*
+ * Orthogonalised matrices (no reference counterpart: the reference's
+ * parameters are rows, not matrices).  For each of batch matrices u
+ * [rows, cols], contiguous: X = u / (|u|_F + eps), and `steps` (1..64) times,
+ * on the short side,  A = X X^T,  X <- a X + (b A + c A^2) X.
+ * orthogonalize takes u = g and writes X to out, both of value_type (0 float,
+ * 1 bf16, 2 fp16); out may be g.
+ * orthogonal_update is one optimizer step:
+ *   momentum = beta momentum + one_minus_beta grad;
+ *   u = nesterov ? one_minus_beta grad + beta momentum : momentum;
+ *   param = keep param - alpha X(u)
+ * with float param and momentum and a grad of value_type.
+ * rows, cols <= 32768.  The coefficients have to keep the singular values
+ * below 1.85 and |a + b s^2 + c s^4| below 7.8, which is checked.  A matrix of
+ * zeros gives zeros, one with a NaN or an infinity NaN throughout; the
+ * matrices of a batch do not touch each other.  workspace: device buffer of
+ * blitz_orthogonalize_workspace_bytes(batch, rows, cols) bytes (0: none
+ * needed), 256-byte aligned, any contents; calls that may run at the same
+ * time need their own.
+ */
+size_t blitz_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols);
+int blitz_orthogonalize(const void* g, int value_type, void* out, int64_t batch, int64_t rows, int64_t cols, int steps,
+                        float a, float b, float c, float eps, void* workspace, size_t workspace_bytes, void* stream);
+int blitz_orthogonal_update(float* param, const void* grad, int value_type, float* momentum, int64_t batch,
+                            int64_t rows, int64_t cols, int steps, float a, float b, float c, float eps, float beta,
+                            float one_minus_beta, int nesterov, float keep, float alpha, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/*
  * Send-buffer packing of one camera's exchange records (no reference
  * counterpart: the reference gathers with torch index_select per rank).
  * Row j < n_rows of records/dest_mask goes to every rank r with bit r set,
