@@ -32,13 +32,12 @@ __device__ __forceinline__ uint32_t row_key(uint32_t seed, int64_t row) {
   return k ^ (k >> 16);
 }
 
-// 20 random bits in [0, 1): x / step has at most 20 bits below one where the
-// format is normal, so the sum before the floor is exact there
-__device__ __forceinline__ float uniform20(uint32_t key, uint32_t col) {
+// 20 random bits
+__device__ __forceinline__ uint32_t random20(uint32_t key, uint32_t col) {
   uint32_t h = key + col * 0x9E3779B1u;
   h = (h ^ (h >> 15)) * 0x2C1B3C6Du;
   h = h ^ (h >> 12);
-  return (float)(h >> 12) * 0x1p-20f;
+  return h >> 12;
 }
 
 // the group's scale, and what x is multiplied by (e4m3) before it is rounded
@@ -61,37 +60,48 @@ __device__ __forceinline__ float inverse_pow2(float s) {
   return s > 0.0f ? __int_as_float((254 << 23) - __float_as_int(s)) : 0.0f;
 }
 
-// x -> code.  s: the group's scale; inv: inverse_pow2(s) (e4m3 only).
+// What the codes of one group are formed with.
+template <int KIND>
+struct GroupCode {
+  float s, inv;    // the scale; inverse_pow2(s) (e4m3 only)
+  uint32_t limit;  // largest magnitude code: 448, or 240 where 256 s would be past the largest float
+  __device__ __forceinline__ explicit GroupCode(float scale)
+      : s(scale), inv(KIND == kE4m3 ? inverse_pow2(scale) : 0.0f), limit(scale >= 0x1p120f ? 0x77u : 0x7eu) {}
+};
+
+// x -> code; r20: random20 (dithered only).
+//
+// An e4m3 magnitude's 7 bits are the top of the float |y| * 2^-120: the
+// exponents then agree, and below 2^-6 both formats count in equal steps (the
+// float's are denormal).  The 20 bits behind them are the fraction of a step,
+// so dithering is an integer addition of 20 random bits; the multiplication
+// rounds towards zero, which does not change floor(fraction + u).
 template <int KIND, bool DITHER, bool NEVER_ZERO = false>
-__device__ __forceinline__ uint8_t encode(float x, float s, float inv, float u) {
+__device__ __forceinline__ uint8_t encode(float x, const GroupCode<KIND>& g, uint32_t r20) {
   if (KIND == kInt8) {
     // a true division, so that the rounding is of x / s itself
-    const float y = s > 0.0f ? __fdiv_rn(x, s) : 0.0f;
-    const float q = DITHER ? floorf(__fadd_rn(y, u)) : rintf(y);
+    const float y = g.s > 0.0f ? __fdiv_rn(x, g.s) : 0.0f;
+    const float q = DITHER ? floorf(__fadd_rn(y, __int_as_float(0x3f800000 | (r20 << 3)) - 1.0f)) : rintf(y);
     return (uint8_t)(int8_t)(int)fminf(fmaxf(q, -127.0f), 127.0f);
   } else {
-    float y = __fmul_rn(x, inv);
-    if (DITHER) {
-      const float mag = fabsf(y);
-      // step = 2^(floor(log2 mag) - 3), 2^-9 below the normal numbers
-      const int b = max(__float_as_int(mag) & 0x7f800000, 121 << 23);
-      const float inv_step = __int_as_float((254 << 23) + (3 << 23) - b);
-      const float q = floorf(__fadd_rn(__fmul_rn(mag, inv_step), u));
-      y = copysignf(__fmul_rn(q, __int_as_float(b - (3 << 23))), y);
-    }
+    const float y = __fmul_rn(x, g.inv);
+    uint32_t code;
+    if (DITHER)
+      code = ((uint32_t)__float_as_int(__fmul_rz(fabsf(y), 0x1p-120f)) + r20) >> 20;
+    else
+      code = (uint32_t)__nv_cvt_float_to_fp8(fabsf(y), __NV_SATFINITE, __NV_E4M3);
+    code = min(code, g.limit);
     // where x > 0, the smallest code at least (x is never negative there)
-    if (NEVER_ZERO) y = x > 0.0f ? fmaxf(y, 0x1p-9f) : y;
-    // 256 * 2^120 is past the largest float: 240 is the code below it
-    if (s >= 0x1p120f) y = fminf(fmaxf(y, -240.0f), 240.0f);
-    return (uint8_t)__nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+    if (NEVER_ZERO) code = x > 0.0f ? max(code, 1u) : code;
+    return (uint8_t)(code | ((uint32_t)__float_as_int(x) >> 24 & 0x80u));
   }
 }
 
 template <int KIND>
 __device__ __forceinline__ float decode(uint8_t c, float s) {
   if (KIND == kInt8) return __fmul_rn((float)(int8_t)c, s);
-  const __half_raw h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)c, __NV_E4M3);
-  return __fmul_rn(__half2float(__half(h)), s);
+  const uint32_t bits = ((uint32_t)c & 0x7fu) << 20 | ((uint32_t)c & 0x80u) << 24;
+  return __fmul_rn(__fmul_rn(__int_as_float((int)bits), 0x1p120f), s);
 }
 
 __device__ __forceinline__ float to_float(float x) { return x; }

@@ -37,8 +37,9 @@ def _round_e4m3(y, u, never_zero):
     with np.errstate(divide="ignore"):
         e = np.where(mag > 0, np.frexp(mag)[1] - 1, -6)
     step = np.ldexp(np.float32(1), np.maximum(e, -6) - 3).astype(np.float32)
-    z = (mag / step).astype(np.float32)
-    q = np.rint(z) if u is None else np.floor((z + u).astype(np.float32))
+    z = mag.astype(np.float64) / step
+    q = np.rint(z) if u is None else np.floor(z + u)
+    q = q.astype(np.float32)
     v = np.copysign((q * step).astype(np.float32), y)
     return np.where(y > 0, np.maximum(v, np.float32(2.0 ** -9)), v) if never_zero else v
 
