@@ -23,7 +23,7 @@
 // (in 64 bits, in a fixed order); `ortho_kernel` is one persistent cooperative
 // block an SM that runs all 3 * steps products with a grid-wide barrier
 // between them, so a step costs no launch.  In it one warp copies tiles of
-// 64 columns by TMA (128-byte swizzle), one thread issues the products, and
+// 64 columns by TMA (128-byte swizzle), one warp issues the products, and
 // eight warps move finished tiles out of tensor memory; tensor memory holds
 // two accumulators, so the next tile's products run meanwhile.  Every wait
 // gives up after two seconds: the outputs are then NaN.
@@ -32,6 +32,7 @@
 #include <algorithm>
 
 #include "ortho.cuh"
+#include "tcgen05.cuh"
 
 namespace blitz {
 
@@ -44,7 +45,6 @@ constexpr int kMaxStages = 6;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 128 + 32 * kEpiWarps;  // warps 0: copies, 1: products, 2: tensor memory, 4..: tiles out
 constexpr int kAcc = 256;                  // tensor-memory columns of one accumulator
-constexpr float kScaleX = 16384.0f, kScaleA = 16384.0f, kScaleB = 8192.0f;
 constexpr int kMaxParts = 256;
 
 struct Info {       // one matrix's scaling, written while X_0 is laid out
@@ -65,96 +65,6 @@ struct KernelParams {
   int two_steps;          // steps 0 .. two_steps-1 use two terms
   int bn_s, bn_x;         // tile widths of the symmetric products and of B X
 };
-
-// ---- PTX wrappers --------------------------------------------------------
-
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.b32 %0, 1, 0, p;\n}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ uint64_t now_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-  return t;
-}
-constexpr uint64_t kGiveUpNs = 2000000000ull;
-
-// false: gave up (or another thread of the block has)
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
-  if (mbar_try(bar, parity)) return true;
-  const uint64_t t0 = now_ns();
-  while (!mbar_try(bar, parity)) {
-    if (*dead) return false;
-    if (now_ns() - t0 > kGiveUpNs) {
-      *dead = 1;
-      return false;
-    }
-  }
-  return true;
-}
-
-__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
-      "[%5];" ::"r"(dst),
-      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
-      : "memory");
-}
-
-// shared-memory matrix descriptor, 128-byte swizzle
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t leading, uint32_t stride) {
-  return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)(leading >> 4) << 16 | (uint64_t)(stride >> 4) << 32 |
-         1ull << 46 | 2ull << 61;
-}
-// f16 x f16 -> f32, M = 128; b_mn: B lies in memory with n contiguous
-__device__ __forceinline__ uint32_t instruction_desc(int bn, bool b_mn) {
-  return 1u << 4 | (b_mn ? 1u << 16 : 0u) | (uint32_t)(bn >> 3) << 17 | (uint32_t)(kBM >> 4) << 24;
-}
-__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
-      : "memory");
-}
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
-  uint32_t r[32];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(addr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
-__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async;" ::: "memory"); }
-__device__ __forceinline__ void tcgen05_before_sync() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tcgen05_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
 // ---- tiles ---------------------------------------------------------------
 
@@ -219,24 +129,14 @@ __device__ __forceinline__ void tile_of(const PhaseShape& s, int t, int& b, int&
   ni = r;
 }
 
-__device__ __forceinline__ uint32_t pack2(__half x, __half y) {
-  return (uint32_t)__half_as_ushort(x) | (uint32_t)__half_as_ushort(y) << 16;
-}
-
 // 32 values of one row as terms at dst (and, the low ones, at dst + low): 16-byte stores
 __device__ __forceinline__ void store_row(__half* dst, int64_t low, const float (&v)[32], bool two) {
 #pragma unroll
   for (int k = 0; k < 32; k += 8) {
-    uint32_t h[4], l[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float x = v[k + 2 * e], y = v[k + 2 * e + 1];
-      const __half hx = __float2half_rn(x), hy = __float2half_rn(y);
-      h[e] = pack2(hx, hy);
-      l[e] = pack2(__float2half_rn(x - __half2float(hx)), __float2half_rn(y - __half2float(hy)));
-    }
-    *(uint4*)(dst + k) = make_uint4(h[0], h[1], h[2], h[3]);
-    if (two) *(uint4*)(dst + low + k) = make_uint4(l[0], l[1], l[2], l[3]);
+    uint4 h, l;
+    split8(v + k, h, l);
+    *(uint4*)(dst + k) = h;
+    if (two) *(uint4*)(dst + low + k) = l;
   }
 }
 
@@ -353,15 +253,16 @@ __global__ void __launch_bounds__(256) prepare_kernel(OrthoParams o, double* par
 
 // every block of the grid has arrived, and what each wrote (for its reads and its copies) is seen
 __device__ bool grid_barrier(const KernelParams& p, unsigned target, volatile int* dead) {
-  fence_async();
+  fence_async_global();
+  fence_async_shared();
   __syncthreads();
   if (threadIdx.x == 0) {
     __threadfence();
     atomicAdd(p.barrier, 1u);
-    const uint64_t t0 = now_ns();
+    const long long t0 = clock64();
     volatile unsigned* arrived = p.barrier;
     while (*arrived < target) {
-      if (*dead || ((volatile unsigned*)p.barrier)[1] || now_ns() - t0 > kGiveUpNs) {
+      if (*dead || ((volatile unsigned*)p.barrier)[1] || clock64() - t0 > kGiveUp) {
         *dead = 1;
         break;
       }
@@ -370,7 +271,8 @@ __device__ bool grid_barrier(const KernelParams& p, unsigned target, volatile in
     __threadfence();
   }
   __syncthreads();
-  fence_async();
+  fence_async_global();
+  fence_async_shared();
   return *dead == 0;
 }
 
@@ -393,13 +295,8 @@ __device__ void lay_out(const KernelParams& p, float* tile) {
         for (int k = threadIdx.x; k < p.n_parts; k += 32) sq += p.parts[b * p.n_parts + k];
 #pragma unroll
         for (int k = 16; k > 0; k >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, k);
-        const double norm = sqrt(sq);
-        // up brings |u|_F to [2^13, 2^14]; u itself keeps its bits
-        int e = norm > 0.0 && norm <= 1e300 ? 14 - (ilogb(norm) + 1) : 0;
-        e = max(-126, min(120, e));
         if (threadIdx.x == 0) {
-          info.up = ldexpf(1.0f, e);
-          info.alpha = (float)(1.0 / ((norm + (double)o.eps) * ldexp(1.0, e)));
+          ortho_scaling(sqrt(sq), o.eps, info.up, info.alpha);
           if (r == 0) p.info[b] = info;
         }
       }
@@ -427,12 +324,10 @@ __device__ void lay_out(const KernelParams& p, float* tile) {
       }
       x *= info.up;
       y *= info.up;
-      const __half hx = __float2half_rn(x), hy = __float2half_rn(y);
       __half* dst = p.x[0] + ((2 * b) * n + i) * (int64_t)p.ldm + j;
-      *(uint32_t*)dst = pack2(hx, hy);
-      if (p.two_in)
-        *(uint32_t*)(dst + (int64_t)n * p.ldm) =
-            pack2(__float2half_rn(x - __half2float(hx)), __float2half_rn(y - __half2float(hy)));
+      uint32_t lo;
+      *(uint32_t*)dst = split2(x, y, lo);
+      if (p.two_in) *(uint32_t*)(dst + (int64_t)n * p.ldm) = lo;
     }
     __syncthreads();
   }
@@ -445,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
   __shared__ int dead_flag;
   volatile int* dead = &dead_flag;
   uint8_t* ring = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t full = smem_addr(bars), empty = full + 8 * kMaxStages, acc_full = full + 16 * kMaxStages,
                  acc_empty = acc_full + 16, ring_addr = smem_addr(ring);
   if (threadIdx.x == 0) {
@@ -460,12 +355,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 2) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)),
-                 "r"(2 * kAcc)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
+  if (warp == 2) tmem_alloc(&tmem_base, 2 * kAcc);
   tcgen05_before_sync();
   __syncthreads();
   tcgen05_after_sync();
@@ -509,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
             }
         }
       }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
       const bool mn = s.which == kApply;
       const uint32_t idesc = instruction_desc(s.bn, mn);
       // 16 of K further: 32 bytes along a row, or 16 rows of 128 bytes
@@ -567,15 +457,14 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_kernel(const __grid_constan
   __syncthreads();
   if (dead_flag) {
     // copies and products of this block that are still in flight end within this time
-    const uint64_t t0 = now_ns();
-    while (now_ns() - t0 < 1000000ull) __nanosleep(1000);
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000ll) __nanosleep(1000);
     const int64_t size = p.o.batch * p.o.n * p.o.m;
     for (int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x; e < size; e += (int64_t)gridDim.x * kThreads)
       ortho_store(p.o, e, __int_as_float(0x7fffffff));
   }
   __syncthreads();
-  if (warp == 2)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kAcc) : "memory");
+  if (warp == 2) tmem_free(tmem, 2 * kAcc);
 }
 
 // ---- host ----------------------------------------------------------------
@@ -654,10 +543,11 @@ int64_t symmetric_tiles(int64_t n, int bn) {
 
 }  // namespace
 
-size_t ortho_workspace_bytes(const OrthoParams& p) { return ortho_small_fits(p) ? 0 : plan_of(p).total; }
+size_t ortho_workspace_bytes(const OrthoParams& p) { return ortho_small_fits(p) || ortho_resident_fits(p) ? 0 : plan_of(p).total; }
 
 int launch_ortho(const OrthoParams& o, void* workspace, cudaStream_t st) {
   if (ortho_small_fits(o)) return launch_ortho_small(o, st);
+  if (ortho_resident_fits(o)) return launch_ortho_resident(o, st);
   int dev = 0, sms = 0;
   if (cudaError_t e = cudaGetDevice(&dev)) return (int)e;
   if (cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) return (int)e;
@@ -676,8 +566,8 @@ int launch_ortho(const OrthoParams& o, void* workspace, cudaStream_t st) {
   p.n_parts = q.n_parts;
   p.ldm = q.ldm;
   p.ldn = q.ldn;
-  p.two_in = o.param != nullptr || o.g_type == kValueF32;
-  p.two_steps = !o.param && o.g_type == kValueBf16 ? std::max(o.steps - 2, 0) : o.steps;
+  p.two_in = ortho_two_in(o);
+  p.two_steps = ortho_two_steps(o);
   p.bn_s = pick_width(o.batch * symmetric_tiles(o.n, 64), o.batch * symmetric_tiles(o.n, 128),
                       o.batch * symmetric_tiles(o.n, 256), sms);
   const int64_t mt = (o.n + kBM - 1) / kBM;

@@ -1,5 +1,7 @@
 // Reading an update and writing its direction, shared by the orthogonalisation kernels.
 #pragma once
+#include <type_traits>
+
 #include "kernels.h"
 #include "ortho.h"
 #include "quant.cuh"
@@ -10,6 +12,48 @@ __device__ __forceinline__ float ortho_g(const OrthoParams& p, int64_t at) {
   if (p.g_type == kValueF32) return ((const float*)p.g)[at];
   if (p.g_type == kValueBf16) return __bfloat162float(((const __nv_bfloat16*)p.g)[at]);
   return __half2float(((const __half*)p.g)[at]);
+}
+
+// the powers of two that X, A and B are scaled by in f16 terms (see ortho.cu)
+constexpr float kScaleX = 16384.0f, kScaleA = 16384.0f, kScaleB = 8192.0f;
+
+// how u with 2-norm `norm` is scaled into f16: it is stored as u * up, exactly,
+// with norm * up in [2^13, 2^14), and X_0 is alpha times that
+__device__ __forceinline__ void ortho_scaling(double norm, float eps, float& up, float& alpha) {
+  int e = norm > 0.0 && norm <= 1e300 ? 14 - (ilogb(norm) + 1) : 0;
+  e = max(-126, min(120, e));
+  up = ldexpf(1.0f, e);
+  alpha = (float)(1.0 / ((norm + (double)eps) * ldexp(1.0, e)));
+}
+
+// whether u needs two f16 terms, and how many steps use two
+__host__ __device__ inline bool ortho_two_in(const OrthoParams& p) { return p.param || p.g_type == kValueF32; }
+__host__ __device__ inline int ortho_two_steps(const OrthoParams& p) {
+  return !p.param && p.g_type == kValueBf16 ? (p.steps > 2 ? p.steps - 2 : 0) : p.steps;
+}
+
+// two values' high terms and, in lo, low ones (one conversion makes a pair)
+__device__ __forceinline__ uint32_t split2(float x, float y, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+  lo = *(const uint32_t*)&l;
+  return *(const uint32_t*)&h;
+}
+// two values from their terms
+__device__ __forceinline__ float2 join2(uint32_t hi, uint32_t lo) {
+  const float2 h = __half22float2(*(const __half2*)&hi), l = __half22float2(*(const __half2*)&lo);
+  return make_float2(h.x + l.x, h.y + l.y);
+}
+// 8 values as 8 high terms and 8 low ones
+__device__ __forceinline__ void split8(const float* v, uint4& hi, uint4& lo) {
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    h[e] = split2(v[2 * e], v[2 * e + 1], l[e]);
+  }
+  hi = make_uint4(h[0], h[1], h[2], h[3]);
+  lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
 // the matrix to be orthogonalised at `at`; the momentum is advanced where this
@@ -27,9 +71,142 @@ __device__ __forceinline__ float ortho_u(const OrthoParams& p, int64_t at) {
   return p.nesterov ? __fadd_rn(g, __fmul_rn(M, p.beta)) : M;
 }
 
-__device__ __forceinline__ void ortho_store(const OrthoParams& p, int64_t at, float o) {
+// V neighbouring values from memory, in 32 bits (V = 4: aligned to 4 of them)
+template <int V>
+__device__ __forceinline__ void load_values(const float* p, float (&v)[V]) {
+  if constexpr (V == 4) {
+    const float4 q = *(const float4*)p;
+    v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+  } else {
+    v[0] = *p;
+  }
+}
+template <int V, class T>
+__device__ __forceinline__ void load_values(const T* p, float (&v)[V]) {
+  if constexpr (V == 4) {
+    const uint2 q = *(const uint2*)p;
+    const T* t = (const T*)&q;
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = quant::to_float(t[k]);
+  } else {
+    v[0] = quant::to_float(*p);
+  }
+}
+template <int V>
+__device__ __forceinline__ void store_values(float* p, const float (&v)[V]) {
+  if constexpr (V == 4)
+    *(float4*)p = make_float4(v[0], v[1], v[2], v[3]);
+  else
+    *p = v[0];
+}
+template <int V, class T>
+__device__ __forceinline__ void store_values(T* p, const float (&v)[V]) {
+  if constexpr (V == 4) {
+    T t[4];
+#pragma unroll
+    for (int k = 0; k < V; ++k) t[k] = quant::from_float<T>(v[k]);
+    *(uint2*)p = *(const uint2*)t;
+  } else {
+    *p = quant::from_float<T>(v[0]);
+  }
+}
+
+// whether a matrix can be taken 4 neighbouring values at a time
+inline bool ortho_by_four(const OrthoParams& p) {
+  const int64_t inner = p.sj == 1 ? p.m : p.n;
+  const uintptr_t wide = (uintptr_t)p.momentum | (uintptr_t)p.param | (p.g_type == kValueF32 ? (uintptr_t)p.g | (uintptr_t)p.out : 0);
+  const uintptr_t narrow = (uintptr_t)p.g | (uintptr_t)p.out;
+  return inner % 4 == 0 && wide % 16 == 0 && narrow % 8 == 0;
+}
+
+// f(position, u) for groups of V values of u at first, first + step, ... below `end`,
+// K groups loaded before the first is used.  T: type of g; UPDATE: with momentum and
+// parameter; ADVANCE: this reading advances the momentum.  (Types are template arguments
+// of the kernels: six variants of this in one kernel cost it 1 KB of spills a thread.)
+template <class T, bool UPDATE, bool ADVANCE, int V, int K, class F>
+__device__ __forceinline__ void ortho_for_u(const OrthoParams& p, int64_t base, int first, int step, int end, F f) {
+  const bool need_g = !UPDATE || ADVANCE || p.nesterov;
+  const T* g = (const T*)p.g + base;
+  float* M = p.momentum + base;
+#pragma unroll 1
+  for (int e0 = first; e0 < end; e0 += K * step) {
+    float u[K][V], old[K][V];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int e = e0 + k * step;
+      if (e < end) {
+        if (need_g) load_values<V>(g + e, u[k]);
+        if (UPDATE) load_values<V>(M + e, old[k]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int e = e0 + k * step;
+      if (e < end) {
+        if (UPDATE) {
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            const float h = need_g ? __fmul_rn(u[k][v], p.one_minus_beta) : 0.0f;
+            if (ADVANCE) old[k][v] = __fadd_rn(__fmul_rn(old[k][v], p.beta), h);
+            u[k][v] = p.nesterov ? __fadd_rn(h, __fmul_rn(old[k][v], p.beta)) : old[k][v];
+          }
+          if (ADVANCE) store_values<V>(M + e, old[k]);
+        }
+        f(e, u[k]);
+      }
+    }
+  }
+}
+
+// Directions o(position, values) written out at first, first + step, ... below `end`:
+// to out, or along them into the parameter.
+template <class T, bool UPDATE, int V, int K, class F>
+__device__ __forceinline__ void ortho_for_out(const OrthoParams& p, int64_t base, int first, int step, int end, F o) {
+  float* q = p.param + base;
+  T* out = (T*)p.out + base;
+#pragma unroll 1
+  for (int e0 = first; e0 < end; e0 += K * step) {
+    float old[K][V];
+    if (UPDATE) {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (e0 + k * step < end) load_values<V>(q + e0 + k * step, old[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int e = e0 + k * step;
+      if (e < end) {
+        float d[V];
+        o(e, d);
+        if (UPDATE) {
+#pragma unroll
+          for (int v = 0; v < V; ++v) d[v] = __fmaf_rn(-p.alpha, d[v], __fmul_rn(old[k][v], p.keep));
+          store_values<V>(q + e, d);
+        } else {
+          store_values<V>(out + e, d);
+        }
+      }
+    }
+  }
+}
+
+// f(type tag, is an update) for a call's types
+template <class F>
+inline auto ortho_dispatch(const OrthoParams& p, F f) {
+  if (p.momentum) {
+    if (p.g_type == kValueF32) return f(float(), std::true_type());
+    if (p.g_type == kValueBf16) return f(__nv_bfloat16(), std::true_type());
+    return f(__half(), std::true_type());
+  }
+  if (p.g_type == kValueF32) return f(float(), std::false_type());
+  if (p.g_type == kValueBf16) return f(__nv_bfloat16(), std::false_type());
+  return f(__half(), std::false_type());
+}
+
+// old: the parameter there, where there is one
+__device__ __forceinline__ void ortho_store(const OrthoParams& p, int64_t at, float o, float old) {
   if (p.param) {
-    p.param[at] = __fmaf_rn(-p.alpha, o, __fmul_rn(p.param[at], p.keep));
+    p.param[at] = __fmaf_rn(-p.alpha, o, __fmul_rn(old, p.keep));
   } else if (p.g_type == kValueF32) {
     ((float*)p.out)[at] = o;
   } else if (p.g_type == kValueBf16) {
@@ -37,6 +214,10 @@ __device__ __forceinline__ void ortho_store(const OrthoParams& p, int64_t at, fl
   } else {
     ((__half*)p.out)[at] = __float2half_rn(o);
   }
+}
+
+__device__ __forceinline__ void ortho_store(const OrthoParams& p, int64_t at, float o) {
+  ortho_store(p, at, o, p.param ? p.param[at] : 0.0f);
 }
 
 }  // namespace blitz

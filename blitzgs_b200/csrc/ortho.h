@@ -28,5 +28,8 @@ int launch_ortho(const OrthoParams& p, void* workspace, cudaStream_t st);
 // ortho_small.cu: matrices that one thread group or one block holds
 bool ortho_small_fits(const OrthoParams& p);
 int launch_ortho_small(const OrthoParams& p, cudaStream_t st);
+// ortho_resident.cu: matrices that one block holds, on the tensor cores
+bool ortho_resident_fits(const OrthoParams& p);
+int launch_ortho_resident(const OrthoParams& p, cudaStream_t st);
 
 }  // namespace blitz

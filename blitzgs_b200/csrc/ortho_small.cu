@@ -19,6 +19,7 @@ namespace blitz {
 namespace {
 
 constexpr int kThinCols = 16;  // columns a lane holds
+constexpr size_t kSharedMost = 200 * 1024;
 
 template <int N, int LANES>
 __global__ void __launch_bounds__(128) thin_kernel(OrthoParams p) {
@@ -266,21 +267,20 @@ int thin(const OrthoParams& p, cudaStream_t st) {
 template <int THREADS>
 int block(const OrthoParams& p, cudaStream_t st) {
   const size_t bytes = block_layout((int)p.n, (int)p.m).bytes;
+  // one value for every size: calls of other threads set the same
   cudaError_t e = cudaFuncSetAttribute(block_kernel<THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)bytes);
+                                       (int)kSharedMost);
   if (e != cudaSuccess) return (int)e;
   const int64_t blocks = std::min<int64_t>(p.batch, 1 << 20);
   block_kernel<THREADS><<<(unsigned)blocks, THREADS, bytes, st>>>(p);
   return (int)cudaGetLastError();
 }
 
-constexpr size_t kSharedMost = 200 * 1024;
-
 }  // namespace
 
 bool ortho_small_fits(const OrthoParams& p) {
   if (p.n <= 4 && p.m <= 32 * kThinCols) return true;
-  return p.n <= 64 && p.m <= 4096 && block_layout((int)p.n, (int)p.m).bytes <= kSharedMost;
+  return p.n <= 16 && p.m <= 4096 && block_layout((int)p.n, (int)p.m).bytes <= kSharedMost;
 }
 
 int launch_ortho_small(const OrthoParams& p, cudaStream_t st) {
