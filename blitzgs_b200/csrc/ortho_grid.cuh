@@ -1,0 +1,81 @@
+// What the orthogonalisation kernels that spread over the grid share: the
+// scratch, the phases of a step and the barrier between them.
+#pragma once
+#include "ortho.cuh"
+#include "tcgen05.cuh"
+
+namespace blitz {
+
+constexpr int kBK = 64;                    // k of one copied box
+constexpr int kBox = 64 * kBK * 2;         // its bytes: 64 rows of 128 bytes
+
+struct OrthoInfo {  // one matrix's scaling, written while X_0 is laid out
+  float up, alpha;  // X_0 is stored as u * up; alpha = 1 / ((|u|_F + eps) * up)
+};
+
+struct OrthoGrid {
+  OrthoParams o;
+  CUtensorMap map_x[2], map_a, map_b;
+  __half *x[2], *a, *b;   // [2 * batch][n][ld]: high and low terms of each matrix
+  double* parts;          // [batch][n_parts] sums of squares
+  OrthoInfo* info;        // [batch]
+  unsigned* barrier;      // [0]: arrivals, [1]: gave up
+  int n_parts;
+  int ldm, ldn;
+  int two_in;             // u needs two terms
+  int two_steps;          // steps 0 .. two_steps - 1 use two terms
+  int four;               // ortho_by_four
+};
+
+enum OrthoPhase : int { kGram, kPoly, kApply };
+
+// which terms a phase reads and writes
+struct OrthoTerms {
+  int which, step;
+  bool two, two_a, two_b, write_two, last;
+  const CUtensorMap *ma, *mb;
+};
+__device__ __forceinline__ OrthoTerms ortho_terms(const OrthoGrid& p, int ph) {
+  OrthoTerms t;
+  t.step = ph / 3;
+  t.which = ph - 3 * t.step;
+  t.two = t.step < p.two_steps;
+  const bool two_x = t.two && (t.step > 0 || p.two_in);
+  t.two_a = t.which == kGram ? two_x : t.two;
+  t.two_b = t.which == kPoly ? t.two : two_x;
+  // A and B are read by this step's own products, the new X by the next one's
+  t.write_two = t.which == kApply ? t.step + 1 < p.two_steps : t.two;
+  t.last = t.step == p.o.steps - 1 && t.which == kApply;
+  t.ma = t.which == kGram ? &p.map_x[t.step & 1] : t.which == kPoly ? &p.map_a : &p.map_b;
+  t.mb = t.which == kPoly ? &p.map_a : &p.map_x[t.step & 1];
+  return t;
+}
+
+// every block of the grid has arrived, and what each wrote (for its reads and its copies) is seen
+__device__ __forceinline__ bool ortho_barrier(unsigned* counter, unsigned target, volatile int* dead) {
+  fence_async_global();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(counter) : "memory");
+    const long long t0 = clock64();
+    for (;;) {
+      unsigned seen;
+      asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(counter) : "memory");
+      if (seen >= target) break;
+      if (*dead || clock64() - t0 > kGiveUp || ((volatile unsigned*)counter)[1]) {
+        *dead = 1;
+        break;
+      }
+    }
+    if (*dead) atomicExch(counter + 1, 1u);
+  }
+  __syncthreads();
+  fence_async_global();
+  return *dead == 0;
+}
+
+int launch_ortho_split(const OrthoGrid& p, int split, cudaStream_t st);
+// the split that launch_ortho_split takes for this size (0: the other kernel), and its clusters
+int ortho_split_for(const OrthoGrid& p, int sms);
+
+}  // namespace blitz

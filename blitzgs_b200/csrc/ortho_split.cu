@@ -1,0 +1,477 @@
+// Orthogonalisation of matrices of medium size over the whole grid (see
+// ortho.cu for the formula, the terms and the phases).
+//
+// A matrix of 1024 rows has 36 symmetric tiles of 128 x 128 for 148 SMs, and an
+// SM takes in about 64 bytes a cycle: 1 MB of operands for one tile's two terms
+// would take 9 us. So a cluster of S blocks shares a tile: each
+// copies and multiplies 1/S of its k, hands the columns that are another's to that
+// block's shared memory, and finishes 1/S of the columns.  Order of the sum: by block, so
+// the result does not depend on timing.
+//
+// Tensor memory holds four accumulators. Where two terms are used each takes
+// one k of 64 (the low terms first) and is then added up in registers: the tensor cores'
+// additions drop the bits below the accumulator's last one, those here round. Over
+// 1024 columns that is the difference between an error of 4e-5 and of 3e-6.
+#include <algorithm>
+
+#include "ortho_grid.cuh"
+
+namespace blitz {
+
+namespace {
+
+constexpr int kB = 128;                       // tiles are kB x kB
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 128 + 32 * kEpiWarps;  // warps 0: copies, 1: products, 2: tensor memory, 4..: tiles out
+constexpr int kAccs = 4;
+constexpr int kRing = 16 * kBox;              // 128 KB
+constexpr int kMaxStages = 4;
+constexpr int kExchange = kB * kB * 4;        // 64 KB
+
+struct Shape {
+  OrthoTerms t;
+  int mt, nt, per, total;  // per: tiles of one matrix
+  int k0, k1;              // this block's k, in boxes
+  int chunk;               // boxes of one accumulator
+  int stage_bytes, stages;
+};
+
+template <int S>
+__device__ __forceinline__ Shape shape_of(const OrthoGrid& p, int ph, int rank) {
+  Shape s;
+  s.t = ortho_terms(p, ph);
+  const int n = (int)p.o.n, m = (int)p.o.m;
+  s.mt = (n + kB - 1) / kB;
+  s.nt = (m + kB - 1) / kB;
+  s.per = s.t.which == kApply ? s.mt * s.nt : s.mt * (s.mt + 1) / 2;
+  s.total = s.per * (int)p.o.batch;
+  const int boxes = ((s.t.which == kGram ? m : n) + kBK - 1) / kBK;
+  s.k0 = boxes * rank / S;
+  s.k1 = boxes * (rank + 1) / S;
+  s.chunk = s.t.two ? 1 : max(s.k1 - s.k0, 1);
+  s.stage_bytes = ((s.t.two_a ? 2 : 1) + (s.t.two_b ? 2 : 1)) * 2 * kBox;
+  s.stages = min(kRing / s.stage_bytes, kMaxStages);
+  return s;
+}
+
+__device__ __forceinline__ void tile_of(const Shape& s, int t, int& b, int& mi, int& ni) {
+  b = t / s.per;
+  const int r = t - b * s.per;
+  if (s.t.which == kApply) {
+    ni = r / s.mt;
+    mi = r - ni * s.mt;
+    return;
+  }
+  // r = mi (mi + 1) / 2 + ni
+  mi = (int)((sqrtf(8.0f * (float)r + 1.0f) - 1.0f) * 0.5f);
+  while (mi * (mi + 1) / 2 > r) --mi;
+  while ((mi + 1) * (mi + 2) / 2 <= r) ++mi;
+  ni = r - mi * (mi + 1) / 2;
+}
+
+// C finished sums of one row (columns col ..) turned into what the phase writes
+template <int C>
+__device__ __forceinline__ void finish(const OrthoGrid& p, const OrthoTerms& t, int b, int row, int col, bool diagonal,
+                                       bool mirror, float (&v)[C]) {
+  const int n = (int)p.o.n, m = (int)p.o.m, lane = threadIdx.x & 31;
+  const float fx = t.step == 0 ? p.info[b].alpha : 1.0f / kScaleX;
+  if (t.which == kApply) {
+    const float f = t.last ? fx / kScaleB : fx * (kScaleX / kScaleB);
+#pragma unroll
+    for (int k = 0; k < C; ++k) v[k] *= f;
+    if (row >= n) return;
+    if (!t.last) {
+      __half* dst = p.x[(t.step + 1) & 1] + ((int64_t)(2 * b) * n + row) * p.ldm + col;
+      const int64_t low = (int64_t)n * p.ldm;
+#pragma unroll
+      for (int k = 0; k < C; k += 8) {
+        if (col + k >= m) break;
+        uint4 hi, lo;
+        split8(v + k, hi, lo);
+        *(uint4*)(dst + k) = hi;
+        if (t.write_two) *(uint4*)(dst + low + k) = lo;
+      }
+      return;
+    }
+    const int64_t at = (int64_t)b * n * m + row * p.o.si;
+    if (p.o.sj == 1 && p.four) {
+#pragma unroll
+      for (int k = 0; k < C; k += 4) {
+        if (col + k >= m) break;
+        float d[4] = {v[k], v[k + 1], v[k + 2], v[k + 3]};
+        const int64_t e = at + col + k;
+        if (p.o.param) {
+          float old[4];
+          load_values<4>(p.o.param + e, old);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) d[q] = __fmaf_rn(-p.o.alpha, d[q], __fmul_rn(old[q], p.o.keep));
+          store_values<4>(p.o.param + e, d);
+        } else if (p.o.g_type == kValueF32) {
+          store_values<4>((float*)p.o.out + e, d);
+        } else if (p.o.g_type == kValueBf16) {
+          store_values<4>((__nv_bfloat16*)p.o.out + e, d);
+        } else {
+          store_values<4>((__half*)p.o.out + e, d);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < C; ++k)
+        if (col + k < m) ortho_store(p.o, at + (col + k) * p.o.sj, v[k]);
+    }
+    return;
+  }
+  const int64_t low = (int64_t)n * p.ldn;
+  if (t.which == kGram) {
+    const float f = fx * fx * kScaleA;
+#pragma unroll
+    for (int k = 0; k < C; ++k) v[k] *= f;
+  } else {
+    // B = a I + b A + c A^2, scaled; A from its terms
+    const float fc = p.o.c * (kScaleB / (kScaleA * kScaleA)), fb = p.o.b * (kScaleB / kScaleA);
+    const __half* A = p.a + ((int64_t)(2 * b) * n + min(row, n - 1)) * p.ldn + col;
+#pragma unroll
+    for (int k = 0; k < C; k += 8) {
+      uint4 h = make_uint4(0, 0, 0, 0), l = h;
+      if (col + k < n) {
+        h = *(const uint4*)(A + k);
+        if (t.two_a) l = *(const uint4*)(A + low + k);
+      }
+      const uint32_t hs[4] = {h.x, h.y, h.z, h.w}, ls[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 x = join2(hs[e], ls[e]);
+        v[k + 2 * e] = fmaf(fc, v[k + 2 * e], fb * x.x);
+        v[k + 2 * e + 1] = fmaf(fc, v[k + 2 * e + 1], fb * x.y);
+      }
+    }
+    if (diagonal) {
+#pragma unroll
+      for (int k = 0; k < C; ++k) v[k] += col + k == row ? p.o.a * kScaleB : 0.0f;
+    }
+  }
+  __half* out = (t.which == kGram ? p.a : p.b) + (int64_t)(2 * b) * n * p.ldn;
+  uint32_t h[C / 2], l[C / 2];
+#pragma unroll
+  for (int k = 0; k < C / 2; ++k) h[k] = split2(v[2 * k], v[2 * k + 1], l[k]);
+  if (row < n) {
+    __half* dst = out + (int64_t)row * p.ldn + col;
+#pragma unroll
+    for (int k = 0; k < C / 2; k += 4) {
+      if (col + 2 * k >= n) break;
+      *(uint4*)(dst + 2 * k) = make_uint4(h[k], h[k + 1], h[k + 2], h[k + 3]);
+      if (t.write_two) *(uint4*)(dst + low + 2 * k) = make_uint4(l[k], l[k + 1], l[k + 2], l[k + 3]);
+    }
+  }
+  if (!mirror) return;
+  // the mirror image: neighbouring lanes (rows) swap halves, so that each writes two
+  // rows' values of one column in one word
+  const int even = row & ~1;
+  __half* to = out + (int64_t)(col + (lane & 1)) * p.ldn + even;
+  const uint32_t pick = lane & 1 ? 0x3276u : 0x5410u;
+#pragma unroll
+  for (int k = 0; k < C / 2; ++k) {
+    const uint32_t ho = __shfl_xor_sync(0xffffffffu, h[k], 1), lo = __shfl_xor_sync(0xffffffffu, l[k], 1);
+    // even lane: (mine.first, other's first); odd lane: (other's second, mine.second)
+    const uint32_t hw = __byte_perm(h[k], ho, pick), lw = __byte_perm(l[k], lo, pick);
+    // ldn is even, so a pair that begins below n stays inside its row
+    if (even < n) {
+      *(uint32_t*)(to + (int64_t)(2 * k) * p.ldn) = hw;
+      if (t.write_two) *(uint32_t*)(to + (int64_t)(2 * k) * p.ldn + low) = lw;
+    }
+  }
+}
+
+template <int S>
+__global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constant__ OrthoGrid p) {
+  extern __shared__ uint8_t raw[];
+  __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 2 * kAccs + 2];
+  __shared__ uint32_t tmem_base;
+  __shared__ int dead_flag;
+  volatile int* dead = &dead_flag;
+  uint8_t* ring = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const uint32_t full = smem_addr(bars), empty = full + 8 * kMaxStages, acc_full = full + 16 * kMaxStages,
+                 acc_empty = acc_full + 8 * kAccs, x_full = acc_empty + 8 * kAccs, x_empty = x_full + 8;
+  const uint32_t ring_addr = smem_addr(ring), exchange = ring_addr + kRing;
+  const int rank = S > 1 ? (int)cluster_rank() : 0;
+  const int first = blockIdx.x / S, by = gridDim.x / S;
+  if (threadIdx.x == 0) {
+    dead_flag = 0;
+    for (int i = 0; i < kMaxStages; ++i) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, 1);
+    }
+    for (int i = 0; i < kAccs; ++i) {
+      mbar_init(acc_full + 8 * i, 1);
+      mbar_init(acc_empty + 8 * i, kEpiWarps);
+    }
+    mbar_init(x_full, kEpiWarps * S);
+    mbar_init(x_empty, kEpiWarps * S);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    for (int i = 0; i < 2; ++i) prefetch_map(&p.map_x[i]);
+    prefetch_map(&p.map_a);
+    prefetch_map(&p.map_b);
+  }
+  if (warp == 2) tmem_alloc(&tmem_base, kAccs * kB);
+  tcgen05_before_sync();
+  __syncthreads();
+  tcgen05_after_sync();
+  if (S > 1) cluster_sync();
+  const uint32_t tmem = tmem_base;
+
+  // each role's parities, one bit a stage or accumulator; a fresh barrier's
+  // "empty" counts as passed, hence the ones
+  uint32_t ph_full = 0, ph_empty = ~0u, ph_accf = 0, ph_acce = ~0u, ph_xf = 0, ph_xe = 1;
+  uint32_t acc_no = 0;
+  unsigned arrivals = 0;
+  bool alive = true;
+  const int phases = 3 * p.o.steps;
+#pragma unroll 1
+  for (int ph = 0; alive && ph < phases; ++ph) {
+    const Shape s = shape_of<S>(p, ph, rank);
+    uint32_t st = 0;
+    if (warp == 0) {
+      for (int t = first; t < s.total && !*dead; t += by) {
+        int b, mi, ni;
+        tile_of(s, t, b, mi, ni);
+        for (int k = s.k0; k < s.k1; ++k) {
+          if (!mbar_wait(empty + 8 * st, ph_empty >> st & 1, dead)) break;
+          ph_empty ^= 1u << st;
+          const uint32_t bar = full + 8 * st;
+          uint32_t dst = ring_addr + st * s.stage_bytes;
+          mbar_expect(bar, s.stage_bytes);
+          for (int term = 0; term < (s.t.two_a ? 2 : 1); ++term)
+            for (int q = 0; q < 2; ++q, dst += kBox) tma_load(dst, s.t.ma, k * kBK, mi * kB + q * 64, 2 * b + term, bar);
+          for (int term = 0; term < (s.t.two_b ? 2 : 1); ++term)
+            for (int q = 0; q < 2; ++q, dst += kBox) {
+              const int at = ni * kB + q * 64;
+              if (s.t.which == kApply)
+                tma_load(dst, s.t.mb, at, k * kBK, 2 * b + term, bar);
+              else
+                tma_load(dst, s.t.mb, k * kBK, at, 2 * b + term, bar);
+            }
+          st = st + 1 == (uint32_t)s.stages ? 0 : st + 1;
+        }
+      }
+    } else if (warp == 1) {
+      const bool mn = s.t.which == kApply;
+      const uint32_t idesc = instruction_desc(kB, mn);
+      // 16 of k further, in units of 16 bytes: 32 bytes along a row, or 16 rows
+      const uint32_t b_step = mn ? 128 : 2, b_lead = mn ? kBox : 16;
+      for (int t = first; t < s.total && !*dead; t += by) {
+        for (int k = s.k0; k < s.k1;) {
+          const uint32_t ac = acc_no;
+          acc_no = (acc_no + 1) % kAccs;
+          if (!mbar_wait(acc_empty + 8 * ac, ph_acce >> ac & 1, dead)) break;
+          ph_acce ^= 1u << ac;
+          tcgen05_after_sync();
+          const uint32_t d = tmem + ac * kB;
+          const int end = min(k + s.chunk, s.k1);
+          uint32_t add = 0;
+          for (; k < end; ++k) {
+            if (!mbar_wait(full + 8 * st, ph_full >> st & 1, dead)) break;
+            ph_full ^= 1u << st;
+            tcgen05_after_sync();
+            const uint32_t a0 = ring_addr + st * s.stage_bytes, b0 = a0 + (s.t.two_a ? 4 : 2) * kBox;
+            for (int q = 0; q < 3; ++q) {
+              // low * high, high * low, high * high
+              if (q == 0 && !s.t.two_a || q == 1 && !s.t.two_b) continue;
+              const uint64_t da = smem_desc(a0 + (q == 0 ? 2 * kBox : 0), 16, 1024);
+              const uint64_t db = smem_desc(b0 + (q == 1 ? 2 * kBox : 0), b_lead, 1024);
+#pragma unroll
+              for (int kk = 0; kk < kBK / 16; ++kk) {
+                mma(d, da + 2 * kk, db + b_step * kk, idesc, add);
+                add = 1;
+              }
+            }
+            mma_commit(empty + 8 * st);
+            st = st + 1 == (uint32_t)s.stages ? 0 : st + 1;
+          }
+          mma_commit(acc_full + 8 * ac);
+        }
+      }
+    } else if (warp >= 4) {
+      const int quarter = warp & 3, half = (warp >> 2) - 1;
+      const uint32_t rows = tmem + ((uint32_t)(quarter * 32) << 16) + half * 64;
+      for (int t = first; t < s.total && !*dead; t += by) {
+        float acc[64];
+#pragma unroll
+        for (int i = 0; i < 64; ++i) acc[i] = 0.0f;
+        bool ok = true;
+        for (int k = s.k0; k < s.k1; k += s.chunk) {
+          const uint32_t ac = acc_no;
+          acc_no = (acc_no + 1) % kAccs;
+          ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * ac, ph_accf >> ac & 1, dead));
+          if (!ok) break;
+          ph_accf ^= 1u << ac;
+          tcgen05_after_sync();
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            float v[32];
+            tmem_load32(rows + ac * kB + g * 32, v);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) acc[g * 32 + i] += v[i];
+          }
+          tcgen05_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(acc_empty + 8 * ac);
+        }
+        if (!ok) break;
+        int b, mi, ni;
+        tile_of(s, t, b, mi, ni);
+        const int local = quarter * 32 + lane, row = mi * kB + local;
+        const bool sym = s.t.which != kApply, diagonal = sym && mi == ni, mirror = sym && mi > ni;
+        if constexpr (S == 1) {
+          finish<64>(p, s.t, b, row, ni * kB + half * 64, diagonal, mirror, acc);
+        } else {
+          constexpr int W = kB / S, C = W / 2;  // columns a block, a thread finishes
+          // the buffer at every block: [from][W / 4 columns][128 rows] of 4 columns' sums
+          ok = __all_sync(0xffffffffu, mbar_wait_cluster(x_empty, ph_xe, dead));
+          if (!ok) break;
+          ph_xe ^= 1;
+#pragma unroll
+          for (int g = 0; g < 16; ++g) {
+            const int c = half * 64 + g * 4, to = c / W, w4 = c % W / 4;
+            peer_store4(peer_addr(exchange + ((rank * (W / 4) + w4) * kB + local) * 16, to),
+                        make_float4(acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]));
+          }
+          __syncwarp();
+          if (lane < S) peer_arrive(peer_addr(x_full, lane));
+          ok = __all_sync(0xffffffffu, mbar_wait_cluster(x_full, ph_xf, dead));
+          if (!ok) break;
+          ph_xf ^= 1;
+          float v[C];
+#pragma unroll
+          for (int i = 0; i < C; ++i) v[i] = 0.0f;
+          const float4* got = (const float4*)(ring + kRing);
+#pragma unroll
+          for (int from = 0; from < S; ++from)
+#pragma unroll
+            for (int g = 0; g < C / 4; ++g) {
+              const float4 x = got[(from * (W / 4) + half * (C / 4) + g) * kB + local];
+              v[4 * g] += x.x;
+              v[4 * g + 1] += x.y;
+              v[4 * g + 2] += x.z;
+              v[4 * g + 3] += x.w;
+            }
+          __syncwarp();
+          if (lane < S) peer_arrive(peer_addr(x_empty, lane));
+          finish<C>(p, s.t, b, row, ni * kB + rank * W + half * C, diagonal, mirror, v);
+        }
+      }
+    }
+    __syncwarp();
+    if (ph + 1 < phases) {
+      arrivals += gridDim.x;
+      alive = ortho_barrier(p.barrier, arrivals, dead);
+    }
+  }
+  __syncthreads();
+  if (dead_flag) {
+    // copies and products of this block that are still in flight end within this time
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000ll) __nanosleep(1000);
+    const int64_t size = p.o.batch * p.o.n * p.o.m;
+    for (int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x; e < size; e += (int64_t)gridDim.x * kThreads)
+      ortho_store(p.o, e, __int_as_float(0x7fffffff));
+  }
+  __syncthreads();
+  if (warp == 2) tmem_free(tmem, kAccs * kB);
+  // a peer may still write to or arrive at this block's shared memory
+  if (S > 1) cluster_sync();
+}
+
+constexpr int kSharedBytes = kRing + kExchange + 1024;
+
+template <int S>
+int configure(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, int blocks, cudaStream_t st) {
+  if (cudaError_t e = cudaFuncSetAttribute(split_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedBytes))
+    return (int)e;
+  cfg = cudaLaunchConfig_t{};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSharedBytes;
+  cfg.stream = st;
+  attr[0].id = cudaLaunchAttributeCooperative;
+  attr[0].val.cooperative = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = S;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return 0;
+}
+
+// clusters of S blocks that fit the device at once
+template <int S>
+int clusters(int sms) {
+  if (S == 1) return sms;
+  static int known[64] = {};  // by device; the same answer whoever asks first
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  if (known[dev] == 0) {
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr[2];
+    int k = 0;
+    if (configure<S>(cfg, attr, S, nullptr)) return 0;
+    cfg.numAttrs = 2;
+    if (cudaOccupancyMaxActiveClusters(&k, split_kernel<S>, &cfg) != cudaSuccess) return 0;
+    known[dev] = std::min(k, sms / S);
+  }
+  return known[dev];
+}
+
+int clusters_of(int split, int sms) {
+  return split == 1 ? clusters<1>(sms) : split == 2 ? clusters<2>(sms) : split == 4 ? clusters<4>(sms) : clusters<8>(sms);
+}
+
+template <int S>
+int start(const OrthoGrid& p, int sms, cudaStream_t st) {
+  const int64_t mt = (p.o.n + kB - 1) / kB, nt = (p.o.m + kB - 1) / kB;
+  const int64_t tiles = p.o.batch * std::max(mt * nt, mt * (mt + 1) / 2);
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr[2];
+  const int k = (int)std::min<int64_t>(clusters<S>(sms), tiles);
+  if (k < 1) return (int)cudaErrorLaunchOutOfResources;
+  if (int rc = configure<S>(cfg, attr, S * k, st)) return rc;
+  return (int)cudaLaunchKernelEx(&cfg, split_kernel<S>, p);
+}
+
+}  // namespace
+
+int ortho_split_for(const OrthoGrid& p, int sms) {
+  const int64_t mt = (p.o.n + kB - 1) / kB, nt = (p.o.m + kB - 1) / kB;
+  const int64_t sym = p.o.batch * mt * (mt + 1) / 2, apply = p.o.batch * mt * nt;
+  const int64_t km = (p.o.m + kBK - 1) / kBK, kn = (p.o.n + kBK - 1) / kBK;
+  int best = 1;
+  double cost = 1e300;
+  for (int s = 1; s <= 8; s *= 2) {
+    const int c = clusters_of(s, sms);
+    if (c < 1) continue;
+    // cycles of a step: rounds of tiles, each a fixed part and one for every box of k
+    auto phase = [&](int64_t tiles, int64_t k) {
+      return (double)((tiles + c - 1) / c) * (2500.0 + (s > 1 ? 1500.0 : 2000.0) + 1300.0 * (double)((k + s - 1) / s));
+    };
+    const double t = phase(sym, km) + phase(sym, kn) + phase(apply, kn);
+    if (t < cost) {
+      cost = t;
+      best = s;
+    }
+  }
+  return best;
+}
+
+int launch_ortho_split(const OrthoGrid& p, int split, cudaStream_t st) {
+  int dev = 0, sms = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return (int)e;
+  if (cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) return (int)e;
+  switch (split) {
+    case 1: return start<1>(p, sms, st);
+    case 2: return start<2>(p, sms, st);
+    case 4: return start<4>(p, sms, st);
+    default: return start<8>(p, sms, st);
+  }
+}
+
+}  // namespace blitz
