@@ -7,7 +7,7 @@
 namespace blitz {
 
 constexpr int kBK = 64;                    // k of one copied box
-constexpr int kBox = 64 * kBK * 2;         // its bytes: 64 rows of 128 bytes
+constexpr int kBox = 64 * kBK * 2;         // bytes of 64 of its rows of 128 bytes
 
 struct OrthoInfo {  // one matrix's scaling, written while X_0 is laid out
   float up, alpha;  // X_0 is stored as u * up; alpha = 1 / ((|u|_F + eps) * up)
@@ -15,7 +15,7 @@ struct OrthoInfo {  // one matrix's scaling, written while X_0 is laid out
 
 struct OrthoGrid {
   OrthoParams o;
-  CUtensorMap map_x[2], map_a, map_b;
+  CUtensorMap map_x[2], map_a, map_b;  // boxes of 64 rows (128 rows a box took a quarter longer)
   __half *x[2], *a, *b;   // [2 * batch][n][ld]: high and low terms of each matrix
   double* parts;          // [batch][n_parts] sums of squares
   OrthoInfo* info;        // [batch]

@@ -5,8 +5,9 @@
 // SM takes in about 64 bytes a cycle: 1 MB of operands for one tile's two terms
 // would take 9 us. So a cluster of S blocks shares a tile: each
 // copies and multiplies 1/S of its k, hands the columns that are another's to that
-// block's shared memory, and finishes 1/S of the columns.  Order of the sum: by block, so
-// the result does not depend on timing.
+// block's shared memory, and finishes 1/S of the columns.  (By bulk copies: stores into a
+// peer's shared memory came to 12 bytes a cycle, 5500 cycles a tile.)  Order of the sum: by
+// block, so the result does not depend on timing.
 //
 // Tensor memory holds four accumulators. Where two terms are used each takes
 // one k of 64 (the low terms first) and is then added up in registers: the tensor cores'
@@ -26,7 +27,9 @@ constexpr int kThreads = 128 + 32 * kEpiWarps;  // warps 0: copies, 1: products,
 constexpr int kAccs = 4;
 constexpr int kRing = 16 * kBox;              // 128 KB
 constexpr int kMaxStages = 4;
-constexpr int kExchange = kB * kB * 4;        // 64 KB
+// columns that go to other blocks, on their way out; and as they come in
+template <int S>
+constexpr int kExchange = (S - 1) * (kB / S) * kB * 4;
 
 struct Shape {
   OrthoTerms t;
@@ -69,10 +72,27 @@ __device__ __forceinline__ void tile_of(const Shape& s, int t, int& b, int& mi, 
   ni = r - mi * (mi + 1) / 2;
 }
 
+// A's terms where a thread will need them for B (read ahead of the sums where there is room)
+template <int C>
+__device__ __forceinline__ void load_a(const OrthoGrid& p, const OrthoTerms& t, int b, int row, int col,
+                                       uint4 (&hi)[C / 8], uint4 (&lo)[C / 8]) {
+  const int n = (int)p.o.n;
+  const __half* A = p.a + ((int64_t)(2 * b) * n + min(row, n - 1)) * p.ldn + col;
+#pragma unroll
+  for (int k = 0; k < C / 8; ++k) {
+    hi[k] = lo[k] = make_uint4(0, 0, 0, 0);
+    if (t.which == kPoly && col + 8 * k < n) {
+      hi[k] = *(const uint4*)(A + 8 * k);
+      if (t.two_a) lo[k] = *(const uint4*)(A + (int64_t)n * p.ldn + 8 * k);
+    }
+  }
+}
+
 // C finished sums of one row (columns col ..) turned into what the phase writes
 template <int C>
 __device__ __forceinline__ void finish(const OrthoGrid& p, const OrthoTerms& t, int b, int row, int col, bool diagonal,
-                                       bool mirror, float (&v)[C]) {
+                                       bool mirror, float (&v)[C], const uint4 (&old_hi)[C / 8],
+                                       const uint4 (&old_lo)[C / 8]) {
   const int n = (int)p.o.n, m = (int)p.o.m, lane = threadIdx.x & 31;
   const float fx = t.step == 0 ? p.info[b].alpha : 1.0f / kScaleX;
   if (t.which == kApply) {
@@ -129,14 +149,9 @@ __device__ __forceinline__ void finish(const OrthoGrid& p, const OrthoTerms& t, 
   } else {
     // B = a I + b A + c A^2, scaled; A from its terms
     const float fc = p.o.c * (kScaleB / (kScaleA * kScaleA)), fb = p.o.b * (kScaleB / kScaleA);
-    const __half* A = p.a + ((int64_t)(2 * b) * n + min(row, n - 1)) * p.ldn + col;
 #pragma unroll
     for (int k = 0; k < C; k += 8) {
-      uint4 h = make_uint4(0, 0, 0, 0), l = h;
-      if (col + k < n) {
-        h = *(const uint4*)(A + k);
-        if (t.two_a) l = *(const uint4*)(A + low + k);
-      }
+      const uint4 h = old_hi[k / 8], l = old_lo[k / 8];
       const uint32_t hs[4] = {h.x, h.y, h.z, h.w}, ls[4] = {l.x, l.y, l.z, l.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -193,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t full = smem_addr(bars), empty = full + 8 * kMaxStages, acc_full = full + 16 * kMaxStages,
                  acc_empty = acc_full + 8 * kAccs, x_full = acc_empty + 8 * kAccs, x_empty = x_full + 8;
-  const uint32_t ring_addr = smem_addr(ring), exchange = ring_addr + kRing;
+  const uint32_t ring_addr = smem_addr(ring), exchange = ring_addr + kRing, incoming = exchange + kExchange<S>;
   const int rank = S > 1 ? (int)cluster_rank() : 0;
   const int first = blockIdx.x / S, by = gridDim.x / S;
   if (threadIdx.x == 0) {
@@ -206,8 +221,8 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
       mbar_init(acc_full + 8 * i, 1);
       mbar_init(acc_empty + 8 * i, kEpiWarps);
     }
-    mbar_init(x_full, kEpiWarps * S);
-    mbar_init(x_empty, kEpiWarps * S);
+    mbar_init(x_full, 1);
+    mbar_init(x_empty, kEpiWarps * (S > 1 ? S - 1 : 1));
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     for (int i = 0; i < 2; ++i) prefetch_map(&p.map_x[i]);
     prefetch_map(&p.map_a);
@@ -292,9 +307,20 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
         }
       }
     } else if (warp >= 4) {
-      const int quarter = warp & 3, half = (warp >> 2) - 1;
-      const uint32_t rows = tmem + ((uint32_t)(quarter * 32) << 16) + half * 64;
-      for (int t = first; t < s.total && !*dead; t += by) {
+      // a block finishes W columns of a tile, a thread C of them in one row: the first or
+      // second half.  It adds up that half of every block's columns.
+      constexpr int W = kB / S, C = W / 2;
+      const int quarter = warp & 3, half = (warp >> 2) - 1, local = quarter * 32 + lane;
+      const uint32_t rows = tmem + ((uint32_t)(quarter * 32) << 16) + half * C;
+      // Warps that gave up go through the rest without waiting (and without arriving): they
+      // meet at a barrier of their own.
+      for (int t = first; t < s.total; t += by) {
+        int b, mi, ni;
+        tile_of(s, t, b, mi, ni);
+        const int row = mi * kB + local, col = ni * kB + rank * W + half * C;
+        const bool sym = s.t.which != kApply, diagonal = sym && mi == ni, mirror = sym && mi > ni;
+        uint4 old_hi[C / 8], old_lo[C / 8];
+        if (S > 1 && s.t.which == kPoly) load_a<C>(p, s.t, b, row, col, old_hi, old_lo);
         float acc[64];
 #pragma unroll
         for (int i = 0; i < 64; ++i) acc[i] = 0.0f;
@@ -302,62 +328,92 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
         for (int k = s.k0; k < s.k1; k += s.chunk) {
           const uint32_t ac = acc_no;
           acc_no = (acc_no + 1) % kAccs;
-          ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * ac, ph_accf >> ac & 1, dead));
-          if (!ok) break;
+          ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * ac, ph_accf >> ac & 1, dead)) && ok;
           ph_accf ^= 1u << ac;
           tcgen05_after_sync();
+          if constexpr (S == 4) {
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            float v[32];
-            tmem_load32(rows + ac * kB + g * 32, v);
+            for (int g = 0; g < 4; ++g) {
+              float v[16];
+              tmem_load16(rows + ac * kB + g * W, v);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) acc[g * 32 + i] += v[i];
+              for (int i = 0; i < 16; ++i) acc[g * 16 + i] += v[i];
+            }
+          } else {
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              float v[32];
+              tmem_load32(rows + ac * kB + g * (S == 1 ? 32 : W), v);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) acc[g * 32 + i] += v[i];
+            }
           }
           tcgen05_before_sync();
           __syncwarp();
-          if (lane == 0) mbar_arrive(acc_empty + 8 * ac);
+          if (lane == 0 && ok) mbar_arrive(acc_empty + 8 * ac);
         }
-        if (!ok) break;
-        int b, mi, ni;
-        tile_of(s, t, b, mi, ni);
-        const int local = quarter * 32 + lane, row = mi * kB + local;
-        const bool sym = s.t.which != kApply, diagonal = sym && mi == ni, mirror = sym && mi > ni;
         if constexpr (S == 1) {
-          finish<64>(p, s.t, b, row, ni * kB + half * 64, diagonal, mirror, acc);
+          load_a<C>(p, s.t, b, row, col, old_hi, old_lo);
+          finish<C>(p, s.t, b, row, col, diagonal, mirror, acc, old_hi, old_lo);
         } else {
-          constexpr int W = kB / S, C = W / 2;  // columns a block, a thread finishes
-          // the buffer at every block: [from][W / 4 columns][128 rows] of 4 columns' sums
-          ok = __all_sync(0xffffffffu, mbar_wait_cluster(x_empty, ph_xe, dead));
-          if (!ok) break;
+          // slots of W / 4 columns x 128 rows of 4 columns' sums; one for each other block, in
+          // the order of their ranks
+          constexpr uint32_t kSlot = W * kB * 4;
+          // what this block sent last has been read, so it has also left
+          ok = __all_sync(0xffffffffu, mbar_wait_cluster(x_empty, ph_xe, dead)) && ok;
           ph_xe ^= 1;
-#pragma unroll
-          for (int g = 0; g < 16; ++g) {
-            const int c = half * 64 + g * 4, to = c / W, w4 = c % W / 4;
-            peer_store4(peer_addr(exchange + ((rank * (W / 4) + w4) * kB + local) * 16, to),
-                        make_float4(acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]));
-          }
-          __syncwarp();
-          if (lane < S) peer_arrive(peer_addr(x_full, lane));
-          ok = __all_sync(0xffffffffu, mbar_wait_cluster(x_full, ph_xf, dead));
-          if (!ok) break;
-          ph_xf ^= 1;
+          float4* out = (float4*)(ring + kRing);
           float v[C];
 #pragma unroll
-          for (int i = 0; i < C; ++i) v[i] = 0.0f;
-          const float4* got = (const float4*)(ring + kRing);
+          for (int to = 0; to < S; ++to) {
+            if (to == rank) {
 #pragma unroll
-          for (int from = 0; from < S; ++from)
+              for (int i = 0; i < C; ++i) v[i] = acc[to * C + i];
+            } else {
+              const int slot = to - (to > rank ? 1 : 0);
 #pragma unroll
-            for (int g = 0; g < C / 4; ++g) {
-              const float4 x = got[(from * (W / 4) + half * (C / 4) + g) * kB + local];
-              v[4 * g] += x.x;
-              v[4 * g + 1] += x.y;
-              v[4 * g + 2] += x.z;
-              v[4 * g + 3] += x.w;
+              for (int g = 0; g < C / 4; ++g)
+                out[(slot * (W / 4) + half * (C / 4) + g) * kB + local] =
+                    make_float4(acc[to * C + 4 * g], acc[to * C + 4 * g + 1], acc[to * C + 4 * g + 2],
+                                acc[to * C + 4 * g + 3]);
             }
+          }
+          fence_async_shared();
+          asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
+          if (warp == 4 && ok) {
+            mbar_expect(x_full, (S - 1) * kSlot);
+#pragma unroll
+            for (int k = 1; k < S; ++k) {
+              const int to = (rank + k) % S, slot = to - (to > rank ? 1 : 0), at = rank - (rank > to ? 1 : 0);
+              peer_copy(peer_addr(incoming + at * kSlot, to), exchange + slot * kSlot, kSlot, peer_addr(x_full, to));
+            }
+          }
+          ok = __all_sync(0xffffffffu, mbar_wait_cluster(x_full, ph_xf, dead)) && ok;
+          ph_xf ^= 1;
+          const float4* got = (const float4*)(ring + kRing + kExchange<S>);
+          float sum[C];
+#pragma unroll
+          for (int i = 0; i < C; ++i) sum[i] = 0.0f;
+#pragma unroll
+          for (int from = 0; from < S; ++from) {
+            if (from == rank) {
+#pragma unroll
+              for (int i = 0; i < C; ++i) sum[i] += v[i];
+            } else {
+              const int slot = from - (from > rank ? 1 : 0);
+#pragma unroll
+              for (int g = 0; g < C / 4; ++g) {
+                const float4 x = got[(slot * (W / 4) + half * (C / 4) + g) * kB + local];
+                sum[4 * g] += x.x;
+                sum[4 * g + 1] += x.y;
+                sum[4 * g + 2] += x.z;
+                sum[4 * g + 3] += x.w;
+              }
+            }
+          }
           __syncwarp();
-          if (lane < S) peer_arrive(peer_addr(x_empty, lane));
-          finish<C>(p, s.t, b, row, ni * kB + rank * W + half * C, diagonal, mirror, v);
+          if (lane < S && lane != rank && ok) peer_arrive(peer_addr(x_empty, lane));
+          finish<C>(p, s.t, b, row, col, diagonal, mirror, sum, old_hi, old_lo);
         }
       }
     }
@@ -382,16 +438,17 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
   if (S > 1) cluster_sync();
 }
 
-constexpr int kSharedBytes = kRing + kExchange + 1024;
+template <int S>
+constexpr int kSharedBytes = kRing + 2 * kExchange<S> + 1024;
 
 template <int S>
 int configure(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, int blocks, cudaStream_t st) {
-  if (cudaError_t e = cudaFuncSetAttribute(split_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedBytes))
+  if (cudaError_t e = cudaFuncSetAttribute(split_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedBytes<S>))
     return (int)e;
   cfg = cudaLaunchConfig_t{};
   cfg.gridDim = dim3((unsigned)blocks);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSharedBytes;
+  cfg.dynamicSmemBytes = kSharedBytes<S>;
   cfg.stream = st;
   attr[0].id = cudaLaunchAttributeCooperative;
   attr[0].val.cooperative = 1;
@@ -423,7 +480,7 @@ int clusters(int sms) {
 }
 
 int clusters_of(int split, int sms) {
-  return split == 1 ? clusters<1>(sms) : split == 2 ? clusters<2>(sms) : split == 4 ? clusters<4>(sms) : clusters<8>(sms);
+  return split == 1 ? clusters<1>(sms) : split == 2 ? clusters<2>(sms) : clusters<4>(sms);
 }
 
 template <int S>
@@ -446,7 +503,7 @@ int ortho_split_for(const OrthoGrid& p, int sms) {
   const int64_t km = (p.o.m + kBK - 1) / kBK, kn = (p.o.n + kBK - 1) / kBK;
   int best = 1;
   double cost = 1e300;
-  for (int s = 1; s <= 8; s *= 2) {
+  for (int s = 1; s <= 4; s *= 2) {
     const int c = clusters_of(s, sms);
     if (c < 1) continue;
     // cycles of a step: rounds of tiles, each a fixed part and one for every box of k
@@ -469,8 +526,7 @@ int launch_ortho_split(const OrthoGrid& p, int split, cudaStream_t st) {
   switch (split) {
     case 1: return start<1>(p, sms, st);
     case 2: return start<2>(p, sms, st);
-    case 4: return start<4>(p, sms, st);
-    default: return start<8>(p, sms, st);
+    default: return start<4>(p, sms, st);
   }
 }
 
