@@ -87,6 +87,7 @@ SIGNATURES = {
 
 _lock = threading.Lock()
 _lib = None
+_entries = {}  # name -> bound entry point
 
 
 def load():
@@ -116,10 +117,12 @@ def exported_symbols():
 
 def call(name, *args):
     """Call an int-returning entry point; raise RuntimeError on a non-zero status."""
-    lib = load()
-    rc = getattr(lib, name)(*args)
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(load(), name)
+    rc = fn(*args)
     if rc != 0:
-        msg = lib.blitz_last_error().decode(errors="replace")
+        msg = load().blitz_last_error().decode(errors="replace")
         raise RuntimeError(f"{name} failed ({rc}): {msg}")
     return rc
 

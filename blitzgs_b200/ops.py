@@ -947,38 +947,47 @@ _CODE_KINDS = {torch.int8: 0, torch.float8_e4m3fn: 1}
 def _same_device(first, *others):
     """All tensors on one GPU, the current device: the launch goes to the
     current device's current stream."""
-    _require_cuda(first, *others)
+    d = first.get_device()
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != d:
+            _require_cuda(first, *others)
             raise RuntimeError(f"tensors on different devices: {first.device} and {t.device}")
-    if first.device.index != torch.cuda.current_device():
+    if d < 0:
+        _require_cuda(first)
+    if d != torch._C._cuda_getDevice():
         raise RuntimeError(f"tensors on {first.device}, but the current device is cuda:{torch.cuda.current_device()}")
 
 
 def _code_rows(codes, scales, group, what):
-    """(N, D) of a store's contiguous codes [N, D] (int8 or float8_e4m3fn) and
-    scales [N, ceil(D / group)]."""
-    if codes.dtype not in _CODE_KINDS:
+    """(N, D, kind) of a store's contiguous codes [N, D] (int8 or
+    float8_e4m3fn) and scales [N, ceil(D / group)]."""
+    kind = _CODE_KINDS.get(codes.dtype)
+    if kind is None:
         raise RuntimeError(f"{what}: codes are int8 or float8_e4m3fn, got {codes.dtype}")
     if scales.dtype != torch.float32 or not codes.is_contiguous() or not scales.is_contiguous():
         raise RuntimeError(f"{what} needs contiguous codes and contiguous float32 scales")
     if not 1 <= group <= 256:
         raise RuntimeError(f"{what}: a group holds 1 to 256 values, got {group}")
-    if codes.dim() != 2 or tuple(scales.shape) != (codes.shape[0], -(-codes.shape[1] // group)):
-        raise RuntimeError(f"{what}: codes {tuple(codes.shape)} in groups of {group} need scales "
-                           f"[{codes.shape[0]}, ceil(D / group)], got {tuple(scales.shape)}")
-    return codes.shape
+    shape = codes.shape
+    if len(shape) != 2 or scales.shape != (shape[0], -(-shape[1] // group)):
+        raise RuntimeError(f"{what}: codes {tuple(shape)} in groups of {group} need scales "
+                           f"[{shape[0]}, ceil(D / group)], got {tuple(scales.shape)}")
+    return shape[0], shape[1], kind
 
 
-def _row_list(rows, device, what):
+def _row_list(rows, what):
     if rows.dim() != 1 or rows.dtype not in (torch.int64, torch.int32):
         raise RuntimeError(f"{what}: rows is a one-dimensional int64 or int32 tensor")
+    if rows.dtype == torch.int64 and rows.is_contiguous():
+        return rows
     return rows.to(torch.int64).contiguous()
 
 
 def _seed(seed, device):
     """A seed as (32-bit integer, device tensor or None): an int64 tensor of
     one element is read by the kernel, so a captured step can count it up."""
+    if type(seed) is int:
+        return seed & 0xFFFFFFFF, None
     if isinstance(seed, torch.Tensor):
         if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != device:
             raise RuntimeError("a seed tensor is one int64 on the same GPU")
@@ -994,19 +1003,20 @@ def quant_rows_write(values, codes, scales, rows=None, *, group, seed=None):
     skipped.  ``seed`` (an int or an int64 tensor of one element) dithers the
     rounding; None rounds to nearest even."""
     _same_device(values, codes, scales, rows)
-    N, D = _code_rows(codes, scales, group, "quant_rows_write")
+    N, D, kind = _code_rows(codes, scales, group, "quant_rows_write")
     n = N if rows is None else rows.numel()
-    if values.dtype not in _VALUE_TYPES or tuple(values.shape) != (n, D):
+    vtype = _VALUE_TYPES.get(values.dtype)
+    if vtype is None or values.shape != (n, D):
         raise RuntimeError(f"quant_rows_write: values of 32 or 16 bits [{n}, {D}] wanted, got {values.dtype} "
                            f"{tuple(values.shape)}")
     if rows is not None:
-        rows = _row_list(rows, codes.device, "quant_rows_write")
+        rows = _row_list(rows, "quant_rows_write")
     if D > 1 and values.stride(1) != 1 or n > 1 and values.stride(0) < D:
         values = values.contiguous()
     s, s_ptr = (0, None) if seed is None else _seed(seed, codes.device)
     tok = TIMER.begin("quant_write")
-    _lib.call("blitz_quant_rows_write", ptr(values), _VALUE_TYPES[values.dtype], values.stride(0) if n > 1 else D,
-              ptr(codes), ptr(scales), _CODE_KINDS[codes.dtype], ptr(rows), n, N, D, int(group),
+    _lib.call("blitz_quant_rows_write", ptr(values), vtype, values.stride(0) if n > 1 else D,
+              ptr(codes), ptr(scales), kind, ptr(rows), n, N, D, int(group),
               int(seed is not None), s, ptr(s_ptr), _lib.stream_ptr())
     TIMER.end(tok, n_rows=n, D=D)
 
@@ -1015,15 +1025,15 @@ def quant_rows_read(codes, scales, rows=None, *, group, dtype=torch.float32):
     """The rows (int64 [n]; None: all) of an 8-bit store as values [n, D] in
     dtype (blitz_quant_rows_read); rows outside [0, N) read as zeros."""
     _same_device(codes, scales, rows)
-    N, D = _code_rows(codes, scales, group, "quant_rows_read")
+    N, D, kind = _code_rows(codes, scales, group, "quant_rows_read")
     if dtype not in _VALUE_TYPES:
         raise RuntimeError(f"quant_rows_read: values are of 32 or 16 bits, got {dtype}")
     if rows is not None:
-        rows = _row_list(rows, codes.device, "quant_rows_read")
+        rows = _row_list(rows, "quant_rows_read")
     n = N if rows is None else rows.numel()
     out = torch.empty((n, D), dtype=dtype, device=codes.device)
     tok = TIMER.begin("quant_read")
-    _lib.call("blitz_quant_rows_read", ptr(codes), ptr(scales), _CODE_KINDS[codes.dtype], ptr(rows), n, N, D,
+    _lib.call("blitz_quant_rows_read", ptr(codes), ptr(scales), kind, ptr(rows), n, N, D,
               int(group), ptr(out), _VALUE_TYPES[dtype], _lib.stream_ptr())
     TIMER.end(tok, n_rows=n, D=D)
     return out
@@ -1037,9 +1047,10 @@ def _adam8(param, grad, m_codes, m_scales, r_codes, r_scales, visible, rows, n, 
     if grad.dtype != torch.float32 or grad.numel() != n * M:
         raise RuntimeError(f"{what} needs a float32 gradient of {n} rows of {M} values")
     for c, s in ((m_codes, m_scales), (r_codes, r_scales)):
-        if tuple(_code_rows(c, s, group, what)) != (N, M) or c.dtype != torch.float8_e4m3fn:
+        if _code_rows(c, s, group, what) != (N, M, 1):
             raise RuntimeError(f"{what} needs float8_e4m3fn moments [{N}, {M}]")
-    grad = grad.contiguous()
+    if not grad.is_contiguous():
+        grad = grad.contiguous()
     s, s_ptr = _seed(seed, param.device)
     tok = TIMER.begin("adam8")
     _lib.call("blitz_adam8_update", ptr(param), ptr(grad), ptr(m_codes), ptr(m_scales), ptr(r_codes), ptr(r_scales),
@@ -1066,7 +1077,7 @@ def adam8_update_rows(param, grad_rows, m_codes, m_scales, r_codes, r_scales, ro
                       seed, grad_scale=1.0):
     """The same step for the Gaussians rows (int64 [n], distinct) whose
     gradients are the rows of grad_rows [n, M]; rows outside [0, N) are skipped."""
-    rows = _row_list(rows, param.device, "adam8_update_rows")
+    rows = _row_list(rows, "adam8_update_rows")
     _adam8(param, grad_rows, m_codes, m_scales, r_codes, r_scales, None, rows, rows.numel(), lr, b1, b2, eps, N, M,
            group, seed, grad_scale, "adam8_update_rows")
 
