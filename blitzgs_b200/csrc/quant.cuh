@@ -69,6 +69,17 @@ struct GroupCode {
       : s(scale), inv(KIND == kE4m3 ? inverse_pow2(scale) : 0.0f), limit(scale >= 0x1p120f ? 0x77u : 0x7eu) {}
 };
 
+// two e4m3 codes -> the numbers they stand for (one conversion makes both)
+__device__ __forceinline__ float2 e4m3_pair(uint8_t x, uint8_t y) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((uint32_t)x | (uint32_t)y << 8), __NV_E4M3);
+  return __half22float2(__half2(h));
+}
+
+// |y| -> magnitude code of y dithered by r20 (see encode)
+__device__ __forceinline__ uint32_t e4m3_dithered(float y, uint32_t r20) {
+  return ((uint32_t)__float_as_int(__fmul_rz(fabsf(y), 0x1p-120f)) + r20) >> 20;
+}
+
 // x -> code; r20: random20 (dithered only).
 //
 // An e4m3 magnitude's 7 bits are the top of the float |y| * 2^-120: the
@@ -87,7 +98,7 @@ __device__ __forceinline__ uint8_t encode(float x, const GroupCode<KIND>& g, uin
     const float y = __fmul_rn(x, g.inv);
     uint32_t code;
     if (DITHER)
-      code = ((uint32_t)__float_as_int(__fmul_rz(fabsf(y), 0x1p-120f)) + r20) >> 20;
+      code = e4m3_dithered(y, r20);
     else
       code = (uint32_t)__nv_cvt_float_to_fp8(fabsf(y), __NV_SATFINITE, __NV_E4M3);
     code = min(code, g.limit);

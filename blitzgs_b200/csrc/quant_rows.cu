@@ -151,9 +151,9 @@ __global__ void __launch_bounds__(256) read_vector_kernel(QuantParams p) {
   }
 }
 
-// One group of one row's step.  The moment updates and the parameter's step
-// are single rounded operations in the order of the formula (no contraction),
-// so the result does not depend on how the compiler fuses them.
+// One group of one row's step.  The moment updates are single rounded operations in
+// the order of the formula (no contraction), so the codes do not depend on how the
+// compiler fuses them.
 template <int LANES, int PER>
 __device__ __forceinline__ void adam8_unit(const Adam8Params& p, int64_t j, int64_t row, int g, int lane,
                                            uint32_t seed) {
@@ -176,27 +176,44 @@ __device__ __forceinline__ void adam8_unit(const Adam8Params& p, int64_t j, int6
   const float ms = row >= 0 ? p.m_scales[sc] : 0.0f, rs = row >= 0 ? p.r_scales[sc] : 0.0f;
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
-    const float g1 = __fmul_rn(w[k], p.grad_scale), root = decode<kE4m3>(r0[k], rs);
-    m[k] = __fadd_rn(__fmul_rn(decode<kE4m3>(m0[k], ms), p.b1), __fmul_rn(g1, p.b1c));
+    const float2 held = e4m3_pair(m0[k], r0[k]);
+    const float g1 = __fmul_rn(w[k], p.grad_scale), root = __fmul_rn(held.y, rs);
+    m[k] = __fadd_rn(__fmul_rn(__fmul_rn(held.x, ms), p.b1), __fmul_rn(g1, p.b1c));
     r[k] = __fsqrt_rn(__fadd_rn(__fmul_rn(__fmul_rn(root, root), p.b2), __fmul_rn(__fmul_rn(g1, g1), p.b2c)));
+    // the quotient to 2 units in its last place: it moves the parameter, whose own rounding
+    // is larger, and the moments' codes do not depend on it
     if (k * LANES < left)
-      param[k * LANES] = __fsub_rn(old[k], __fdiv_rn(__fmul_rn(m[k], p.lr), __fadd_rn(r[k], p.eps)));
+      param[k * LANES] = __fsub_rn(old[k], __fdividef(__fmul_rn(m[k], p.lr), __fadd_rn(r[k], p.eps)));
   }
   const float sm = scale_of<kE4m3, LANES, PER>(m), sr = scale_of<kE4m3, LANES, PER>(r);
   if (row < 0) return;
   const uint32_t km = row_key(seed, row), kr = row_key(seed ^ 0x5BF03635u, row);
-  const GroupCode<kE4m3> gm(sm), gr(sr);
-  const bool okm = sm == sm, okr = sr == sr;
+  const float im = inverse_pow2(sm), ir = inverse_pow2(sr);
+  uint8_t a[PER], b[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const uint32_t col = c0 + lane + k * LANES;
+    a[k] = (uint8_t)(e4m3_dithered(__fmul_rn(m[k], im), random20(km, col)) |
+                     ((uint32_t)__float_as_int(m[k]) >> 24 & 0x80u));
+    // a second moment that has seen a gradient never becomes zero: the next step would
+    // divide its first moment by the new gradient alone (r is not negative, so r > 0
+    // where its bits are not 0)
+    b[k] = (uint8_t)max(e4m3_dithered(__fmul_rn(r[k], ir), random20(kr, col)),
+                        min((uint32_t)__float_as_int(r[k]), 1u));
+  }
+  if (!(sm < 0x1p120f) || !(sr < 0x1p120f)) {
+    // rare: a scale that is not finite, or whose largest code would not be
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      a[k] = sm == sm ? (uint8_t)((a[k] & 0x80u) | min(a[k] & 0x7fu, GroupCode<kE4m3>(sm).limit)) : (uint8_t)0;
+      b[k] = sr == sr ? (uint8_t)min((uint32_t)b[k], GroupCode<kE4m3>(sr).limit) : (uint8_t)0;
+    }
+  }
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
     if (k * LANES < left) {
-      const uint32_t col = c0 + lane + k * LANES;
-      const uint8_t a = encode<kE4m3, true>(m[k], gm, random20(km, col));
-      // a second moment that has seen a gradient never becomes zero: the next
-      // step would divide its first moment by the new gradient alone
-      const uint8_t b = encode<kE4m3, true, true>(r[k], gr, random20(kr, col));
-      mc[k * LANES] = okm ? a : (uint8_t)0;
-      rc[k * LANES] = okr ? b : (uint8_t)0;
+      mc[k * LANES] = a[k];
+      rc[k * LANES] = b[k];
     }
   }
   if (lane == 0) {

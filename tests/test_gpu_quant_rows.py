@@ -1,6 +1,8 @@
 """The 8-bit row store and the sparse Adam step on it, against their numpy
-restatement.  The store's arithmetic is single float32 operations in a fixed
-order, so codes, scales and parameters are compared bit for bit."""
+restatement.  The store's arithmetic and the moments' are single float32 operations in
+a fixed order, so codes and scales are compared bit for bit.  The parameter's step is a
+quotient to 2 units in its last place: against the correctly rounded one, parameters
+differ by at most 2^-22 of the step and one unit (2^-23) of the parameter."""
 import numpy as np
 import pytest
 import torch
@@ -220,8 +222,11 @@ def test_adam8_matches_the_definition(cuda_device, N, M, group, form):
         want, (qm, sm), (qr, sr) = O.adam8(ref, g, O.dequantise(m[0][i], m[1][i], group),
                                            O.dequantise(r[0][i], r[1][i], group), i, lr, 0.9, 0.999, eps, 100 + t,
                                            group)
-        ref[i], m[0][i], m[1][i], r[0][i], r[1][i] = want, qm, sm, qr, sr
-        assert np.array_equal(p.cpu().numpy(), ref)
+        got = p.cpu().numpy()
+        assert (np.abs(got[i] - want) <= 2.0 ** -22 * np.abs(want - ref[i]) + 2.0 ** -23 * np.abs(want)).all()
+        rest = np.setdiff1d(np.arange(N), i)
+        assert np.array_equal(got[rest], ref[rest])
+        ref, m[0][i], m[1][i], r[0][i], r[1][i] = got.copy(), qm, sm, qr, sr
         for got, s, w in ((mc, ms, m), (rc, rs, r)):
             assert np.array_equal(s.cpu().numpy(), w[1])
             assert np.array_equal(_numbers(got), w[0])
