@@ -32,6 +32,18 @@ __host__ __device__ inline int ortho_two_steps(const OrthoParams& p) {
   return !p.param && p.g_type == kValueBf16 ? (p.steps > 2 ? p.steps - 2 : 0) : p.steps;
 }
 
+// 32 bytes of global memory, a whole sector, by one lane
+__device__ __forceinline__ void store32(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+__device__ __forceinline__ void load32(const void* p, uint32_t (&v)[8]) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "l"(p)
+               : "memory");
+}
 // two values' high terms and, in lo, low ones (one conversion makes a pair)
 __device__ __forceinline__ uint32_t split2(float x, float y, uint32_t& lo) {
   const __half2 h = __floats2half2_rn(x, y);

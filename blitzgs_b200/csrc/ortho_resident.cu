@@ -59,24 +59,24 @@ struct Product {
   bool b_mn;             // b lies with n along a row
 };
 
-__device__ __forceinline__ void issue(const Product& q, uint32_t d, uint32_t bar) {
+__device__ __forceinline__ void issue(const Product& q, uint32_t on, uint32_t d, uint32_t bar) {
   const uint32_t idesc = instruction_desc(q.n, q.b_mn);
   uint32_t add = 0;
   for (int t = 0; t < 3; ++t) {
     // low * high, high * low, high * high
     if (t == 0 && !q.two_a || t == 1 && !q.two_b) continue;
-    const uint64_t a0 = smem_desc(q.a + (t == 0 ? q.a_term : 0), 16, 1024);
-    const uint64_t b0 = smem_desc(q.b + (t == 1 ? q.b_term : 0), q.b_mn ? kGroup : 16, 1024);
+    const uint32_t a0 = smem_desc(q.a + (t == 0 ? q.a_term : 0), 16);
+    const uint32_t b0 = smem_desc(q.b + (t == 1 ? q.b_term : 0), q.b_mn ? kGroup : 16);
     // 16 of k further, in units of 16 bytes: 32 bytes along a row, the next 64 columns after
     // four of them, or 16 rows
 #pragma unroll 4
     for (int k = 0; k < q.k; ++k) {
       const uint32_t along = (uint32_t)(k >> 2) * (kGroup >> 4) + (uint32_t)(k & 3) * 2;
-      mma(d, a0 + along, b0 + (q.b_mn ? (uint32_t)k * 128 : along), idesc, add);
+      mma(on, d, a0 + along, b0 + (q.b_mn ? (uint32_t)k * 128 : along), idesc, add);
       add = 1;
     }
   }
-  mma_commit(bar);
+  mma_commit(on, bar);
 }
 
 // position e of a matrix stored in rows of `inner`, without a division a step
@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) resident_kernel(OrthoP
   tcgen05_before_sync();
   __syncthreads();
   tcgen05_after_sync();
-  const uint32_t tmem = tmem_base;
+  const uint32_t tmem = tmem_base, on = elected();
   const int row = (warp & 3) * 32 + lane;
   const uint32_t tmem_rows = tmem + ((uint32_t)((warp & 3) * 32) << 16);
   uint32_t parity = 0;
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) resident_kernel(OrthoP
           q.k = (which == 0 ? l.mp : l.np) / 16;
           q.n = which == 2 ? l.mp : l.np;
           q.b_mn = which == 2;
-          issue(q, tmem, bar);
+          issue(q, on, tmem, bar);
         }
         mbar_wait(bar, parity, dead);
         parity ^= 1;

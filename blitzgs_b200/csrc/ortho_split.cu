@@ -9,6 +9,17 @@
 // peer's shared memory came to 12 bytes a cycle, 5500 cycles a tile.)  Order of the sum: by
 // block, so the result does not depend on timing.
 //
+// Where there are tiles enough (S = 1), shared memory bounds the products: one of 128 x 128 x
+// 16 reads 8 KB of operands in 64 cycles' work and takes 85.  (Tiles of 128 x 256, 12 KB
+// in 128 cycles, have fewer units in flight and leave more SMs without one: 4260 us for 3760
+// at 4096^2. Pairs of blocks on 256 x 128 took 5530.)
+//
+// The operands' ring holds the low terms of a k of 64 and the high ones as units of their own:
+// the low ones are free after two thirds of the products.  Two warps issue copies, every
+// second unit each, and two issue products, every second k of 64 each into accumulators of its
+// own: a wait that is already over still takes 125 cycles, a product's issue 45 and a copy's
+// 100, which one warp each would not hide behind 768 cycles of products.
+//
 // Tensor memory holds four accumulators. Where two terms are used each takes
 // one k of 64 (the low terms first) and is then added up in registers: the tensor cores'
 // additions drop the bits below the accumulator's last one, those here round. Over
@@ -23,20 +34,25 @@ namespace {
 
 constexpr int kB = 128;                       // tiles are kB x kB
 constexpr int kEpiWarps = 8;
-constexpr int kThreads = 128 + 32 * kEpiWarps;  // warps 0: copies, 1: products, 2: tensor memory, 4..: tiles out
-constexpr int kAccs = 4;
-constexpr int kRing = 16 * kBox;              // 128 KB
-constexpr int kMaxStages = 4;
+constexpr int kThreads = 128 + 32 * kEpiWarps;  // warps 0, 1: copies, 2, 3: products, 4..: tiles out
+constexpr int kColumns = 512;                 // of tensor memory: all
+
+constexpr int kAccs = kColumns / kB;
+constexpr int kUnit = 4 * kBox;               // one term of both operands
+template <int S>
+constexpr int kUnits = S == 1 ? 6 : 4;        // 192 or 128 KB; even: a slot's units are one warp's
+template <int S>
+constexpr int kRing = kUnits<S> * kUnit;
 // columns that go to other blocks, on their way out; and as they come in
 template <int S>
-constexpr int kExchange = (S - 1) * (kB / S) * kB * 4;
+constexpr int kExchange = S > 1 ? (S - 1) * (kB / S) * kB * 4 : 0;
 
 struct Shape {
   OrthoTerms t;
   int mt, nt, per, total;  // per: tiles of one matrix
-  int k0, k1;              // this block's k, in boxes
-  int chunk;               // boxes of one accumulator
-  int stage_bytes, stages;
+  int k0, boxes;           // this block's k, in boxes
+  int units;               // units of a box: 2 where an operand has two terms
+  int accs;                // accumulators of a tile: one a box, or one for every second box
 };
 
 template <int S>
@@ -46,14 +62,16 @@ __device__ __forceinline__ Shape shape_of(const OrthoGrid& p, int ph, int rank) 
   const int n = (int)p.o.n, m = (int)p.o.m;
   s.mt = (n + kB - 1) / kB;
   s.nt = (m + kB - 1) / kB;
-  s.per = s.t.which == kApply ? s.mt * s.nt : s.mt * (s.mt + 1) / 2;
+  if (s.t.which == kApply)
+    s.per = s.mt * s.nt;
+  else
+    s.per = s.mt * (s.mt + 1) / 2;
   s.total = s.per * (int)p.o.batch;
   const int boxes = ((s.t.which == kGram ? m : n) + kBK - 1) / kBK;
-  s.k0 = boxes * rank / S;
-  s.k1 = boxes * (rank + 1) / S;
-  s.chunk = s.t.two ? 1 : max(s.k1 - s.k0, 1);
-  s.stage_bytes = ((s.t.two_a ? 2 : 1) + (s.t.two_b ? 2 : 1)) * 2 * kBox;
-  s.stages = min(kRing / s.stage_bytes, kMaxStages);
+  s.k0 = S > 1 ? boxes * rank / S : 0;
+  s.boxes = (S > 1 ? boxes * (rank + 1) / S : boxes) - s.k0;
+  s.units = s.t.two_a || s.t.two_b ? 2 : 1;
+  s.accs = s.t.two ? s.boxes : min(s.boxes, 2);
   return s;
 }
 
@@ -75,24 +93,38 @@ __device__ __forceinline__ void tile_of(const Shape& s, int t, int& b, int& mi, 
 // A's terms where a thread will need them for B (read ahead of the sums where there is room)
 template <int C>
 __device__ __forceinline__ void load_a(const OrthoGrid& p, const OrthoTerms& t, int b, int row, int col,
-                                       uint4 (&hi)[C / 8], uint4 (&lo)[C / 8]) {
+                                       uint32_t (&hi)[C / 2], uint32_t (&lo)[C / 2]) {
   const int n = (int)p.o.n;
   const __half* A = p.a + ((int64_t)(2 * b) * n + min(row, n - 1)) * p.ldn + col;
 #pragma unroll
-  for (int k = 0; k < C / 8; ++k) {
-    hi[k] = lo[k] = make_uint4(0, 0, 0, 0);
-    if (t.which == kPoly && col + 8 * k < n) {
-      hi[k] = *(const uint4*)(A + 8 * k);
-      if (t.two_a) lo[k] = *(const uint4*)(A + (int64_t)n * p.ldn + 8 * k);
+  for (int k = 0; k < C / 2; k += 8) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) hi[k + e] = lo[k + e] = 0;
+    // rows are a whole number of 64 columns long, so 16 from one below n are in the row
+    if (t.which == kPoly && col + 2 * k < n) {
+      load32(A + 2 * k, *(uint32_t(*)[8])(hi + k));
+      if (t.two_a) load32(A + (int64_t)n * p.ldn + 2 * k, *(uint32_t(*)[8])(lo + k));
     }
+  }
+}
+
+// C values' terms to row `dst`, the low ones `low` further, as far as there are columns
+template <int C>
+__device__ __forceinline__ void store_terms(__half* dst, int64_t low, int left, bool two, const uint32_t (&h)[C / 2],
+                                            const uint32_t (&l)[C / 2]) {
+#pragma unroll
+  for (int k = 0; k < C / 2; k += 8) {
+    if (2 * k >= left) break;
+    store32(dst + 2 * k, *(const uint32_t(*)[8])(h + k));
+    if (two) store32(dst + low + 2 * k, *(const uint32_t(*)[8])(l + k));
   }
 }
 
 // C finished sums of one row (columns col ..) turned into what the phase writes
 template <int C>
 __device__ __forceinline__ void finish(const OrthoGrid& p, const OrthoTerms& t, int b, int row, int col, bool diagonal,
-                                       bool mirror, float (&v)[C], const uint4 (&old_hi)[C / 8],
-                                       const uint4 (&old_lo)[C / 8]) {
+                                       bool mirror, float (&v)[C], const uint32_t (&old_hi)[C / 2],
+                                       const uint32_t (&old_lo)[C / 2]) {
   const int n = (int)p.o.n, m = (int)p.o.m, lane = threadIdx.x & 31;
   const float fx = t.step == 0 ? p.info[b].alpha : 1.0f / kScaleX;
   if (t.which == kApply) {
@@ -101,16 +133,11 @@ __device__ __forceinline__ void finish(const OrthoGrid& p, const OrthoTerms& t, 
     for (int k = 0; k < C; ++k) v[k] *= f;
     if (row >= n) return;
     if (!t.last) {
-      __half* dst = p.x[(t.step + 1) & 1] + ((int64_t)(2 * b) * n + row) * p.ldm + col;
-      const int64_t low = (int64_t)n * p.ldm;
+      uint32_t h[C / 2], l[C / 2];
 #pragma unroll
-      for (int k = 0; k < C; k += 8) {
-        if (col + k >= m) break;
-        uint4 hi, lo;
-        split8(v + k, hi, lo);
-        *(uint4*)(dst + k) = hi;
-        if (t.write_two) *(uint4*)(dst + low + k) = lo;
-      }
+      for (int k = 0; k < C / 2; ++k) h[k] = split2(v[2 * k], v[2 * k + 1], l[k]);
+      store_terms<C>(p.x[(t.step + 1) & 1] + ((int64_t)(2 * b) * n + row) * p.ldm + col, (int64_t)n * p.ldm, m - col,
+                     t.write_two, h, l);
       return;
     }
     const int64_t at = (int64_t)b * n * m + row * p.o.si;
@@ -150,15 +177,10 @@ __device__ __forceinline__ void finish(const OrthoGrid& p, const OrthoTerms& t, 
     // B = a I + b A + c A^2, scaled; A from its terms
     const float fc = p.o.c * (kScaleB / (kScaleA * kScaleA)), fb = p.o.b * (kScaleB / kScaleA);
 #pragma unroll
-    for (int k = 0; k < C; k += 8) {
-      const uint4 h = old_hi[k / 8], l = old_lo[k / 8];
-      const uint32_t hs[4] = {h.x, h.y, h.z, h.w}, ls[4] = {l.x, l.y, l.z, l.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 x = join2(hs[e], ls[e]);
-        v[k + 2 * e] = fmaf(fc, v[k + 2 * e], fb * x.x);
-        v[k + 2 * e + 1] = fmaf(fc, v[k + 2 * e + 1], fb * x.y);
-      }
+    for (int k = 0; k < C / 2; ++k) {
+      const float2 x = join2(old_hi[k], old_lo[k]);
+      v[2 * k] = fmaf(fc, v[2 * k], fb * x.x);
+      v[2 * k + 1] = fmaf(fc, v[2 * k + 1], fb * x.y);
     }
     if (diagonal) {
 #pragma unroll
@@ -169,15 +191,7 @@ __device__ __forceinline__ void finish(const OrthoGrid& p, const OrthoTerms& t, 
   uint32_t h[C / 2], l[C / 2];
 #pragma unroll
   for (int k = 0; k < C / 2; ++k) h[k] = split2(v[2 * k], v[2 * k + 1], l[k]);
-  if (row < n) {
-    __half* dst = out + (int64_t)row * p.ldn + col;
-#pragma unroll
-    for (int k = 0; k < C / 2; k += 4) {
-      if (col + 2 * k >= n) break;
-      *(uint4*)(dst + 2 * k) = make_uint4(h[k], h[k + 1], h[k + 2], h[k + 3]);
-      if (t.write_two) *(uint4*)(dst + low + 2 * k) = make_uint4(l[k], l[k + 1], l[k + 2], l[k + 3]);
-    }
-  }
+  if (row < n) store_terms<C>(out + (int64_t)row * p.ldn + col, low, n - col, t.write_two, h, l);
   if (!mirror) return;
   // the mirror image: neighbouring lanes (rows) swap halves, so that each writes two
   // rows' values of one column in one word
@@ -200,20 +214,21 @@ __device__ __forceinline__ void finish(const OrthoGrid& p, const OrthoTerms& t, 
 template <int S>
 __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constant__ OrthoGrid p) {
   extern __shared__ uint8_t raw[];
-  __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 2 * kAccs + 2];
+  __shared__ __align__(8) uint64_t bars[2 * kUnits<S> + 2 * kAccs + 4];
   __shared__ uint32_t tmem_base;
   __shared__ int dead_flag;
   volatile int* dead = &dead_flag;
   uint8_t* ring = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const uint32_t full = smem_addr(bars), empty = full + 8 * kMaxStages, acc_full = full + 16 * kMaxStages,
-                 acc_empty = acc_full + 8 * kAccs, x_full = acc_empty + 8 * kAccs, x_empty = x_full + 8;
-  const uint32_t ring_addr = smem_addr(ring), exchange = ring_addr + kRing, incoming = exchange + kExchange<S>;
+  const uint32_t full = smem_addr(bars), empty = full + 8 * kUnits<S>, acc_full = empty + 8 * kUnits<S>,
+                 acc_empty = acc_full + 8 * kAccs, x_full = acc_empty + 8 * kAccs, x_empty = x_full + 8,
+                 token = x_empty + 8;
+  const uint32_t ring_addr = smem_addr(ring), exchange = ring_addr + kRing<S>, incoming = exchange + kExchange<S>;
   const int rank = S > 1 ? (int)cluster_rank() : 0;
   const int first = blockIdx.x / S, by = gridDim.x / S;
   if (threadIdx.x == 0) {
     dead_flag = 0;
-    for (int i = 0; i < kMaxStages; ++i) {
+    for (int i = 0; i < kUnits<S>; ++i) {
       mbar_init(full + 8 * i, 1);
       mbar_init(empty + 8 * i, 1);
     }
@@ -221,6 +236,7 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
       mbar_init(acc_full + 8 * i, 1);
       mbar_init(acc_empty + 8 * i, kEpiWarps);
     }
+    for (int i = 0; i < 2; ++i) mbar_init(token + 8 * i, 1);
     mbar_init(x_full, 1);
     mbar_init(x_empty, kEpiWarps * (S > 1 ? S - 1 : 1));
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -228,85 +244,105 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
     prefetch_map(&p.map_a);
     prefetch_map(&p.map_b);
   }
-  if (warp == 2) tmem_alloc(&tmem_base, kAccs * kB);
+  if (warp == 0) tmem_alloc(&tmem_base, kColumns);
   tcgen05_before_sync();
   __syncthreads();
   tcgen05_after_sync();
   if (S > 1) cluster_sync();
-  const uint32_t tmem = tmem_base;
+  // all 512 columns are this block's, so they begin at 0 (which the compiler then knows to
+  // be the same for the whole warp)
+  constexpr uint32_t tmem = 0;
+  const uint32_t on = elected();
 
-  // each role's parities, one bit a stage or accumulator; a fresh barrier's
-  // "empty" counts as passed, hence the ones
-  uint32_t ph_full = 0, ph_empty = ~0u, ph_accf = 0, ph_acce = ~0u, ph_xf = 0, ph_xe = 1;
-  uint32_t acc_no = 0;
+  // Units and accumulators are numbered through the whole run, by every role alike: number u
+  // lies in slot u % kUnits and is that slot's use u / kUnits, whose parity is waited for.
+  uint32_t unit0 = 0, acc0 = 0, box0 = 0, ph_xf = 0, ph_xe = 1;
   unsigned arrivals = 0;
   bool alive = true;
   const int phases = 3 * p.o.steps;
 #pragma unroll 1
   for (int ph = 0; alive && ph < phases; ++ph) {
     const Shape s = shape_of<S>(p, ph, rank);
-    uint32_t st = 0;
-    if (warp == 0) {
+    const int tiles = first < s.total ? (s.total - first + by - 1) / by : 0;
+    if (warp < 2) {
+      uint32_t u = unit0;
       for (int t = first; t < s.total && !*dead; t += by) {
         int b, mi, ni;
         tile_of(s, t, b, mi, ni);
-        for (int k = s.k0; k < s.k1; ++k) {
-          if (!mbar_wait(empty + 8 * st, ph_empty >> st & 1, dead)) break;
-          ph_empty ^= 1u << st;
-          const uint32_t bar = full + 8 * st;
-          uint32_t dst = ring_addr + st * s.stage_bytes;
-          mbar_expect(bar, s.stage_bytes);
-          for (int term = 0; term < (s.t.two_a ? 2 : 1); ++term)
-            for (int q = 0; q < 2; ++q, dst += kBox) tma_load(dst, s.t.ma, k * kBK, mi * kB + q * 64, 2 * b + term, bar);
-          for (int term = 0; term < (s.t.two_b ? 2 : 1); ++term)
-            for (int q = 0; q < 2; ++q, dst += kBox) {
-              const int at = ni * kB + q * 64;
-              if (s.t.which == kApply)
-                tma_load(dst, s.t.mb, at, k * kBK, 2 * b + term, bar);
-              else
-                tma_load(dst, s.t.mb, k * kBK, at, 2 * b + term, bar);
-            }
-          st = st + 1 == (uint32_t)s.stages ? 0 : st + 1;
+        for (int k = s.k0; k < s.k0 + s.boxes; ++k) {
+          // the low terms, then the high ones
+          for (int term = s.units - 1; term >= 0; --term, ++u) {
+            if ((u & 1) != (uint32_t)warp) continue;
+            const uint32_t slot = u % kUnits<S>;
+            if (!mbar_wait(empty + 8 * slot, (u / kUnits<S> & 1) ^ 1, dead)) break;
+            const bool has_a = term == 0 || s.t.two_a, has_b = term == 0 || s.t.two_b;
+            const uint32_t bar = full + 8 * slot, dst = ring_addr + slot * kUnit;
+            mbar_expect(on, bar, (has_a ? 2 * kBox : 0) + (has_b ? 2 * kBox : 0));
+            if (has_a)
+              for (int q = 0; q < 2; ++q)
+                tma_load(on, dst + q * kBox, s.t.ma, k * kBK, mi * kB + q * 64, 2 * b + term, bar);
+            if (has_b)
+              for (int q = 0; q < 2; ++q) {
+                const int at = ni * kB + q * 64;
+                if (s.t.which == kApply)
+                  tma_load(on, dst + (2 + q) * kBox, s.t.mb, at, k * kBK, 2 * b + term, bar);
+                else
+                  tma_load(on, dst + (2 + q) * kBox, s.t.mb, k * kBK, at, 2 * b + term, bar);
+              }
+          }
         }
       }
-    } else if (warp == 1) {
+    } else if (warp < 4) {
       const bool mn = s.t.which == kApply;
       const uint32_t idesc = instruction_desc(kB, mn);
       // 16 of k further, in units of 16 bytes: 32 bytes along a row, or 16 rows
       const uint32_t b_step = mn ? 128 : 2, b_lead = mn ? kBox : 16;
-      for (int t = first; t < s.total && !*dead; t += by) {
-        for (int k = s.k0; k < s.k1;) {
-          const uint32_t ac = acc_no;
-          acc_no = (acc_no + 1) % kAccs;
-          if (!mbar_wait(acc_empty + 8 * ac, ph_acce >> ac & 1, dead)) break;
-          ph_acce ^= 1u << ac;
-          tcgen05_after_sync();
-          const uint32_t d = tmem + ac * kB;
-          const int end = min(k + s.chunk, s.k1);
-          uint32_t add = 0;
-          for (; k < end; ++k) {
-            if (!mbar_wait(full + 8 * st, ph_full >> st & 1, dead)) break;
-            ph_full ^= 1u << st;
-            tcgen05_after_sync();
-            const uint32_t a0 = ring_addr + st * s.stage_bytes, b0 = a0 + (s.t.two_a ? 4 : 2) * kBox;
-            for (int q = 0; q < 3; ++q) {
-              // low * high, high * low, high * high
-              if (q == 0 && !s.t.two_a || q == 1 && !s.t.two_b) continue;
-              const uint64_t da = smem_desc(a0 + (q == 0 ? 2 * kBox : 0), 16, 1024);
-              const uint64_t db = smem_desc(b0 + (q == 1 ? 2 * kBox : 0), b_lead, 1024);
-#pragma unroll
-              for (int kk = 0; kk < kBK / 16; ++kk) {
-                mma(d, da + 2 * kk, db + b_step * kk, idesc, add);
-                add = 1;
-              }
-            }
-            mma_commit(empty + 8 * st);
-            st = st + 1 == (uint32_t)s.stages ? 0 : st + 1;
+      // The boxes of the whole run go to the two warps in turn, and a warp waits for one only
+      // when the other has what it waited for before it: a parity cannot tell a barrier two
+      // uses behind from one that is ready.
+      const uint32_t mine = warp - 2;
+      uint32_t u0 = unit0, a0 = acc0, g0 = box0;
+      for (int t = 0; t < tiles && !*dead; ++t, u0 += s.boxes * s.units, a0 += s.accs, g0 += s.boxes) {
+        uint32_t add = 0;
+        for (int k = (int)((mine ^ g0) & 1); k < s.boxes; k += 2) {
+          const uint32_t turn = (g0 + k) >> 1;
+          if (!mbar_wait(token + 8 * mine, (turn + (mine ? 0 : 1)) & 1, dead)) break;
+          const uint32_t a = a0 + (s.t.two ? k : k & 1), d = tmem + a % kAccs * kB;
+          if (s.t.two || k < 2) {
+            if (!mbar_wait(acc_empty + 8 * (a % kAccs), (a / kAccs & 1) ^ 1, dead)) break;
+            add = 0;
           }
-          mma_commit(acc_full + 8 * ac);
+          const uint32_t ul = u0 + k * s.units, uh = ul + s.units - 1;
+          const uint32_t lo = ul % kUnits<S>, hi = uh % kUnits<S>;
+          if (s.units == 2 && !mbar_wait(full + 8 * lo, ul / kUnits<S> & 1, dead)) break;
+          if (!mbar_wait(full + 8 * hi, uh / kUnits<S> & 1, dead)) break;
+          if (lane == 0) mbar_arrive(token + 8 * (mine ^ 1));
+          __syncwarp();
+          tcgen05_after_sync();
+          const uint32_t ah = smem_desc(ring_addr + hi * kUnit, 16),
+                         bh = smem_desc(ring_addr + hi * kUnit + 2 * kBox, b_lead);
+          if (s.units == 2) {
+            const uint32_t al = smem_desc(ring_addr + lo * kUnit, 16),
+                           bl = smem_desc(ring_addr + lo * kUnit + 2 * kBox, b_lead);
+            // low * high, high * low: small terms first
+            if (s.t.two_a) {
+#pragma unroll
+              for (int kk = 0; kk < kBK / 16; ++kk, add = 1) mma(on, d, al + 2 * kk, bh + b_step * kk, idesc, add);
+            }
+            if (s.t.two_b) {
+#pragma unroll
+              for (int kk = 0; kk < kBK / 16; ++kk, add = 1) mma(on, d, ah + 2 * kk, bl + b_step * kk, idesc, add);
+            }
+            mma_commit(on, empty + 8 * lo);
+          }
+#pragma unroll
+          for (int kk = 0; kk < kBK / 16; ++kk, add = 1) mma(on, d, ah + 2 * kk, bh + b_step * kk, idesc, add);
+          mma_commit(on, empty + 8 * hi);
+          if (s.t.two || k + 2 >= s.boxes) mma_commit(on, acc_full + 8 * (a % kAccs));
         }
       }
-    } else if (warp >= 4) {
+    } else {
+      uint32_t a = acc0;
       // a block finishes W columns of a tile, a thread C of them in one row: the first or
       // second half.  It adds up that half of every block's columns.
       constexpr int W = kB / S, C = W / 2;
@@ -317,19 +353,17 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
       for (int t = first; t < s.total; t += by) {
         int b, mi, ni;
         tile_of(s, t, b, mi, ni);
-        const int row = mi * kB + local, col = ni * kB + rank * W + half * C;
+        const int row = mi * kB + local, col = ni * kB + (S > 1 ? rank * W : 0) + half * C;
         const bool sym = s.t.which != kApply, diagonal = sym && mi == ni, mirror = sym && mi > ni;
-        uint4 old_hi[C / 8], old_lo[C / 8];
-        if (S > 1 && s.t.which == kPoly) load_a<C>(p, s.t, b, row, col, old_hi, old_lo);
+        uint32_t old_hi[S > 1 ? C / 2 : 1], old_lo[S > 1 ? C / 2 : 1];
+        if constexpr (S > 1) load_a<C>(p, s.t, b, row, col, old_hi, old_lo);
         float acc[64];
 #pragma unroll
         for (int i = 0; i < 64; ++i) acc[i] = 0.0f;
         bool ok = true;
-        for (int k = s.k0; k < s.k1; k += s.chunk) {
-          const uint32_t ac = acc_no;
-          acc_no = (acc_no + 1) % kAccs;
-          ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * ac, ph_accf >> ac & 1, dead)) && ok;
-          ph_accf ^= 1u << ac;
+        for (int j = 0; j < s.accs; ++j, ++a) {
+          const uint32_t ac = a % kAccs;
+          ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * ac, a / kAccs & 1, dead)) && ok;
           tcgen05_after_sync();
           if constexpr (S == 4) {
 #pragma unroll
@@ -343,7 +377,7 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
               float v[32];
-              tmem_load32(rows + ac * kB + g * (S == 1 ? 32 : W), v);
+              tmem_load32(rows + ac * kB + g * (S == 2 ? W : 32), v);
 #pragma unroll
               for (int i = 0; i < 32; ++i) acc[g * 32 + i] += v[i];
             }
@@ -353,8 +387,15 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
           if (lane == 0 && ok) mbar_arrive(acc_empty + 8 * ac);
         }
         if constexpr (S == 1) {
-          load_a<C>(p, s.t, b, row, col, old_hi, old_lo);
-          finish<C>(p, s.t, b, row, col, diagonal, mirror, acc, old_hi, old_lo);
+#pragma unroll
+          for (int c = 0; c < C; c += 32) {
+            uint32_t hi[16], lo[16];
+            float v[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = acc[c + i];
+            load_a<32>(p, s.t, b, row, col + c, hi, lo);
+            finish<32>(p, s.t, b, row, col + c, diagonal, mirror, v, hi, lo);
+          }
         } else {
           // slots of W / 4 columns x 128 rows of 4 columns' sums; one for each other block, in
           // the order of their ranks
@@ -362,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
           // what this block sent last has been read, so it has also left
           ok = __all_sync(0xffffffffu, mbar_wait_cluster(x_empty, ph_xe, dead)) && ok;
           ph_xe ^= 1;
-          float4* out = (float4*)(ring + kRing);
+          float4* out = (float4*)(ring + kRing<S>);
           float v[C];
 #pragma unroll
           for (int to = 0; to < S; ++to) {
@@ -381,16 +422,16 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
           fence_async_shared();
           asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
           if (warp == 4 && ok) {
-            mbar_expect(x_full, (S - 1) * kSlot);
+            mbar_expect(on, x_full, (S - 1) * kSlot);
 #pragma unroll
             for (int k = 1; k < S; ++k) {
               const int to = (rank + k) % S, slot = to - (to > rank ? 1 : 0), at = rank - (rank > to ? 1 : 0);
-              peer_copy(peer_addr(incoming + at * kSlot, to), exchange + slot * kSlot, kSlot, peer_addr(x_full, to));
+              peer_copy(on, peer_addr(incoming + at * kSlot, to), exchange + slot * kSlot, kSlot, peer_addr(x_full, to));
             }
           }
           ok = __all_sync(0xffffffffu, mbar_wait_cluster(x_full, ph_xf, dead)) && ok;
           ph_xf ^= 1;
-          const float4* got = (const float4*)(ring + kRing + kExchange<S>);
+          const float4* got = (const float4*)(ring + kRing<S> + kExchange<S>);
           float sum[C];
 #pragma unroll
           for (int i = 0; i < C; ++i) sum[i] = 0.0f;
@@ -418,6 +459,9 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
       }
     }
     __syncwarp();
+    unit0 += (uint32_t)(tiles * s.boxes * s.units);
+    box0 += (uint32_t)(tiles * s.boxes);
+    acc0 += (uint32_t)(tiles * s.accs);
     if (ph + 1 < phases) {
       arrivals += gridDim.x;
       alive = ortho_barrier(p.barrier, arrivals, dead);
@@ -433,13 +477,13 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
       ortho_store(p.o, e, __int_as_float(0x7fffffff));
   }
   __syncthreads();
-  if (warp == 2) tmem_free(tmem, kAccs * kB);
+  if (warp == 0) tmem_free(tmem_base, kColumns);
   // a peer may still write to or arrive at this block's shared memory
   if (S > 1) cluster_sync();
 }
 
 template <int S>
-constexpr int kSharedBytes = kRing + 2 * kExchange<S> + 1024;
+constexpr int kSharedBytes = kRing<S> + 2 * kExchange<S> + 1024;
 
 template <int S>
 int configure(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, int blocks, cudaStream_t st) {
@@ -472,7 +516,6 @@ int clusters(int sms) {
     cudaLaunchAttribute attr[2];
     int k = 0;
     if (configure<S>(cfg, attr, S, nullptr)) return 0;
-    cfg.numAttrs = 2;
     if (cudaOccupancyMaxActiveClusters(&k, split_kernel<S>, &cfg) != cudaSuccess) return 0;
     known[dev] = std::min(k, sms / S);
   }
@@ -497,20 +540,24 @@ int start(const OrthoGrid& p, int sms, cudaStream_t st) {
 
 }  // namespace
 
+// The split whose step takes the fewest cycles by a count fitted to what was measured (us for a
+// split of 1 / 2 / 4 in 32 bits: 512^2 168 / 160 / 124, 768^2 193 / 178 / 158, 1024^2 222 / 200 /
+// 222, 1300^2 261 / 285 / 319, 2048^2 458 / 708 / 759): rounds of tiles, each with a fixed part
+// (latencies, the exchange, the tile's end) and one for every box of k.
 int ortho_split_for(const OrthoGrid& p, int sms) {
   const int64_t mt = (p.o.n + kB - 1) / kB, nt = (p.o.m + kB - 1) / kB;
-  const int64_t sym = p.o.batch * mt * (mt + 1) / 2, apply = p.o.batch * mt * nt;
   const int64_t km = (p.o.m + kBK - 1) / kBK, kn = (p.o.n + kBK - 1) / kBK;
+  const int64_t sym = p.o.batch * mt * (mt + 1) / 2, apply = p.o.batch * mt * nt;
+  const struct {
+    int split, fixed, box;
+  } ways[] = {{1, 13000, 870}, {2, 13700, 1250}, {4, 11800, 1250}};
   int best = 1;
-  double cost = 1e300;
-  for (int s = 1; s <= 4; s *= 2) {
-    const int c = clusters_of(s, sms);
+  int64_t cost = INT64_MAX;
+  for (const auto& w : ways) {
+    const int c = clusters_of(w.split, sms), s = w.split;
     if (c < 1) continue;
-    // cycles of a step: rounds of tiles, each a fixed part and one for every box of k
-    auto phase = [&](int64_t tiles, int64_t k) {
-      return (double)((tiles + c - 1) / c) * (2500.0 + (s > 1 ? 1500.0 : 2000.0) + 1300.0 * (double)((k + s - 1) / s));
-    };
-    const double t = phase(sym, km) + phase(sym, kn) + phase(apply, kn);
+    auto phase = [&](int64_t tiles, int64_t k) { return (tiles + c - 1) / c * (w.fixed + w.box * ((k + s - 1) / s)); };
+    const int64_t t = phase(sym, km) + phase(sym, kn) + phase(apply, kn);
     if (t < cost) {
       cost = t;
       best = s;

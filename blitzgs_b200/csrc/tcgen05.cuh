@@ -19,6 +19,12 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// 1 in one lane of a whole warp, always the same one
+__device__ __forceinline__ uint32_t elected() {
+  uint32_t on;
+  asm volatile("{\n .reg .pred e;\n .reg .b32 r;\n elect.sync r|e, 0xffffffff;\n selp.b32 %0, 1, 0, e;\n}" : "=r"(on));
+  return on;
+}
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -46,20 +52,20 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   return true;
 }
 
-// by an elected lane of a whole warp, as the products below
-__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+// by the lane of a whole warp that has `on`, as the products below
+__device__ __forceinline__ void tma_load(uint32_t on, uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
   asm volatile(
-      "{\n .reg .pred e;\n .reg .b32 r;\n elect.sync r|e, 0xffffffff;\n"
+      "{\n .reg .pred e;\n setp.ne.u32 e, %6, 0;\n"
       " @e cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
       "[%5];\n}" ::"r"(dst),
-      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar), "r"(on)
       : "memory");
 }
-__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
+__device__ __forceinline__ void mbar_expect(uint32_t on, uint32_t bar, uint32_t bytes) {
   asm volatile(
-      "{\n .reg .pred e;\n .reg .b32 r;\n elect.sync r|e, 0xffffffff;\n"
+      "{\n .reg .pred e;\n setp.ne.u32 e, %2, 0;\n"
       " @e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}" ::"r"(bar),
-      "r"(bytes)
+      "r"(bytes), "r"(on)
       : "memory");
 }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
@@ -77,12 +83,12 @@ __device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
-// this block's shared memory to a peer's, by an elected lane of a whole warp; bar: the peer's
-__device__ __forceinline__ void peer_copy(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar) {
+// this block's shared memory to a peer's; bar: the peer's
+__device__ __forceinline__ void peer_copy(uint32_t on, uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar) {
   asm volatile(
-      "{\n .reg .pred e;\n .reg .b32 r;\n elect.sync r|e, 0xffffffff;\n"
+      "{\n .reg .pred e;\n setp.ne.u32 e, %4, 0;\n"
       " @e cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n}" ::"r"(dst),
-      "r"(src), "r"(bytes), "r"(bar)
+      "r"(src), "r"(bytes), "r"(bar), "r"(on)
       : "memory");
 }
 __device__ __forceinline__ void peer_arrive(uint32_t bar) {
@@ -114,30 +120,33 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// shared-memory matrix descriptor, 128-byte swizzle
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t leading, uint32_t stride) {
-  return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)(leading >> 4) << 16 | (uint64_t)(stride >> 4) << 32 |
-         1ull << 46 | 2ull << 61;
+// Shared-memory matrix descriptors, 128-byte swizzle, 1024 bytes from one group of 8 rows to
+// the next: the lower word holds the address and the leading stride (both in units of 16
+// bytes), the upper one never changes.
+__device__ __forceinline__ uint32_t smem_desc(uint32_t addr, uint32_t leading) {
+  return ((addr >> 4) & 0x3fff) | (leading >> 4) << 16;
 }
-// f16 x f16 -> f32, M = 128; b_mn: B lies in memory with n contiguous
-__device__ __forceinline__ uint32_t instruction_desc(int bn, bool b_mn) {
-  return 1u << 4 | (b_mn ? 1u << 16 : 0u) | (uint32_t)(bn >> 3) << 17 | (128u >> 4) << 24;
+constexpr uint32_t kDescUpper = (1024u >> 4) | 1u << 14 | 2u << 29;
+// f16 x f16 -> f32; b_mn: B lies in memory with n contiguous
+__device__ __forceinline__ uint32_t instruction_desc(int bn, bool b_mn, uint32_t rows = 128) {
+  return 1u << 4 | (b_mn ? 1u << 16 : 0u) | (uint32_t)(bn >> 3) << 17 | (rows >> 4) << 24;
 }
-// One product and one commit.  The whole warp calls these with the same operands
-// and one elected lane issues: where a branch picks the lane instead, the compiler cannot
-// see that the operands are the same for the warp and spends 180 cycles a product on
-// moving them to uniform registers.
-__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+// One product and one commit (and, above, copies).  The whole warp calls these with the
+// same operands and the lane that has `on` issues: where a branch picks the lane instead, the
+// compiler cannot see that the operands are the same for the warp and spends 180
+// cycles a product on moving them to uniform registers.
+__device__ __forceinline__ void mma(uint32_t on, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t add) {
   asm volatile(
-      "{\n .reg .pred p, e;\n .reg .b32 r;\n elect.sync r|e, 0xffffffff;\n setp.ne.u32 p, %4, 0;\n"
-      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      "{\n .reg .pred p, e;\n .reg .b64 da, db;\n setp.ne.u32 e, %5, 0;\n setp.ne.u32 p, %4, 0;\n"
+      " mov.b64 da, {%1, %6};\n mov.b64 db, {%2, %6};\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(add), "r"(on), "n"(kDescUpper)
       : "memory");
 }
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
+__device__ __forceinline__ void mma_commit(uint32_t on, uint32_t bar) {
   asm volatile(
-      "{\n .reg .pred e;\n .reg .b32 r;\n elect.sync r|e, 0xffffffff;\n"
-      " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(bar)
+      "{\n .reg .pred e;\n setp.ne.u32 e, %1, 0;\n"
+      " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(bar), "r"(on)
       : "memory");
 }
 __device__ __forceinline__ void tmem_alloc(uint32_t* where, int columns) {
