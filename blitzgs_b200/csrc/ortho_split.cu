@@ -143,28 +143,41 @@ __device__ __forceinline__ void finish(const OrthoGrid& p, const OrthoTerms& t, 
     const int64_t at = (int64_t)b * n * m + row * p.o.si;
     if (p.o.sj == 1 && p.four) {
 #pragma unroll
-      for (int k = 0; k < C; k += 4) {
-        if (col + k >= m) break;
-        float d[4] = {v[k], v[k + 1], v[k + 2], v[k + 3]};
-        const int64_t e = at + col + k;
-        if (p.o.param) {
-          float old[4];
-          load_values<4>(p.o.param + e, old);
+      for (int k0 = 0; k0 < C; k0 += 16) {
+        // 16 of the parameter's values before the first of them is written
+        float old[16];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) d[q] = __fmaf_rn(-p.o.alpha, d[q], __fmul_rn(old[q], p.o.keep));
-          store_values<4>(p.o.param + e, d);
-        } else if (p.o.g_type == kValueF32) {
-          store_values<4>((float*)p.o.out + e, d);
-        } else if (p.o.g_type == kValueBf16) {
-          store_values<4>((__nv_bfloat16*)p.o.out + e, d);
-        } else {
-          store_values<4>((__half*)p.o.out + e, d);
+        for (int k = k0; k < k0 + 16; k += 4)
+          if (p.o.param && col + k < m) load_values<4>(p.o.param + at + col + k, *(float(*)[4])(old + k - k0));
+#pragma unroll
+        for (int k = k0; k < k0 + 16; k += 4) {
+          if (col + k >= m) break;
+          float d[4] = {v[k], v[k + 1], v[k + 2], v[k + 3]};
+          const int64_t e = at + col + k;
+          if (p.o.param) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) d[q] = __fmaf_rn(-p.o.alpha, d[q], __fmul_rn(old[k - k0 + q], p.o.keep));
+            store_values<4>(p.o.param + e, d);
+          } else if (p.o.g_type == kValueF32) {
+            store_values<4>((float*)p.o.out + e, d);
+          } else if (p.o.g_type == kValueBf16) {
+            store_values<4>((__nv_bfloat16*)p.o.out + e, d);
+          } else {
+            store_values<4>((__half*)p.o.out + e, d);
+          }
         }
       }
     } else {
 #pragma unroll
-      for (int k = 0; k < C; ++k)
-        if (col + k < m) ortho_store(p.o, at + (col + k) * p.o.sj, v[k]);
+      for (int k0 = 0; k0 < C; k0 += 16) {
+        float old[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          old[k] = p.o.param && col + k0 + k < m ? p.o.param[at + (col + k0 + k) * p.o.sj] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          if (col + k0 + k < m) ortho_store(p.o, at + (col + k0 + k) * p.o.sj, v[k0 + k], old[k]);
+      }
     }
     return;
   }
@@ -355,8 +368,6 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
         tile_of(s, t, b, mi, ni);
         const int row = mi * kB + local, col = ni * kB + (S > 1 ? rank * W : 0) + half * C;
         const bool sym = s.t.which != kApply, diagonal = sym && mi == ni, mirror = sym && mi > ni;
-        uint32_t old_hi[S > 1 ? C / 2 : 1], old_lo[S > 1 ? C / 2 : 1];
-        if constexpr (S > 1) load_a<C>(p, s.t, b, row, col, old_hi, old_lo);
         float acc[64];
 #pragma unroll
         for (int i = 0; i < 64; ++i) acc[i] = 0.0f;
@@ -419,6 +430,9 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
                                 acc[to * C + 4 * g + 3]);
             }
           }
+          // A's terms, while the sums travel
+          uint32_t old_hi[C / 2], old_lo[C / 2];
+          load_a<C>(p, s.t, b, row, col, old_hi, old_lo);
           fence_async_shared();
           asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
           if (warp == 4 && ok) {
