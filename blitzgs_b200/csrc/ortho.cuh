@@ -8,12 +8,6 @@
 
 namespace blitz {
 
-__device__ __forceinline__ float ortho_g(const OrthoParams& p, int64_t at) {
-  if (p.g_type == kValueF32) return ((const float*)p.g)[at];
-  if (p.g_type == kValueBf16) return __bfloat162float(((const __nv_bfloat16*)p.g)[at]);
-  return __half2float(((const __half*)p.g)[at]);
-}
-
 // the powers of two that X, A and B are scaled by in f16 terms (see ortho.cu)
 constexpr float kScaleX = 16384.0f, kScaleA = 16384.0f, kScaleB = 8192.0f;
 
@@ -68,21 +62,6 @@ __device__ __forceinline__ void split8(const float* v, uint4& hi, uint4& lo) {
   lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
-// the matrix to be orthogonalised at `at`; the momentum is advanced where this
-// is its first reading (`advance`), else taken as it stands
-template <bool ADVANCE>
-__device__ __forceinline__ float ortho_u(const OrthoParams& p, int64_t at) {
-  if (!p.momentum) return ortho_g(p, at);
-  float g = 0.0f;
-  if (ADVANCE || p.nesterov) g = __fmul_rn(ortho_g(p, at), p.one_minus_beta);
-  float M = p.momentum[at];
-  if (ADVANCE) {
-    M = __fadd_rn(__fmul_rn(M, p.beta), g);
-    p.momentum[at] = M;
-  }
-  return p.nesterov ? __fadd_rn(g, __fmul_rn(M, p.beta)) : M;
-}
-
 // V neighbouring values from memory, in 32 bits (V = 4: aligned to 4 of them)
 template <int V>
 __device__ __forceinline__ void load_values(const float* p, float (&v)[V]) {
@@ -123,13 +102,14 @@ __device__ __forceinline__ void store_values(T* p, const float (&v)[V]) {
   }
 }
 
-// whether a matrix can be taken 4 neighbouring values at a time
-inline bool ortho_by_four(const OrthoParams& p) {
-  const int64_t inner = p.sj == 1 ? p.m : p.n;
-  const uintptr_t wide = (uintptr_t)p.momentum | (uintptr_t)p.param | (p.g_type == kValueF32 ? (uintptr_t)p.g | (uintptr_t)p.out : 0);
+// whether the tensors begin where 4 neighbouring values can be taken at once, and whether every
+// row does
+inline bool ortho_aligned(const OrthoParams& p) {
   const uintptr_t narrow = (uintptr_t)p.g | (uintptr_t)p.out;
-  return inner % 4 == 0 && wide % 16 == 0 && narrow % 8 == 0;
+  const uintptr_t wide = (uintptr_t)p.momentum | (uintptr_t)p.param | (p.g_type == kValueF32 ? narrow : 0);
+  return wide % 16 == 0 && narrow % 8 == 0;
 }
+inline bool ortho_by_four(const OrthoParams& p) { return (p.sj == 1 ? p.m : p.n) % 4 == 0 && ortho_aligned(p); }
 
 // f(position, u) for groups of V values of u at first, first + step, ... below `end`,
 // K groups loaded before the first is used.  T: type of g; UPDATE: with momentum and

@@ -70,6 +70,16 @@ def test_matches_the_formula(cuda_device, shape, dtype):
         assert _off(got, O.orthogonalize(g.double().numpy())) <= _tol(min(shape), dtype)
 
 
+@pytest.mark.parametrize("shape", [(1030, 1100), (1400, 1290), (1153, 2177), (20, 150, 260), (40, 257, 130),
+                                   (130, 5000), (3, 129, 385)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_many_tiles_and_long_sums(cuda_device, shape, dtype):
+    """Sizes whose tiles are split over clusters or not, with odd numbers of tiles and of k blocks."""
+    g = _input(shape, dtype, form="low")
+    got = ops.orthogonalize(g.to(cuda_device))
+    assert _off(got, O.orthogonalize(g.double().numpy())) <= _tol(min(shape[-2:]), dtype)
+
+
 @pytest.mark.parametrize("shape", [(1000, 15, 3), (37, 3, 4), (50, 16, 16), (5, 40, 24), (7, 130, 70), (3, 2, 64, 200),
                                    (3, 300, 260), (200, 70, 66)])
 def test_matrices_of_a_batch_do_not_touch_each_other(cuda_device, shape):
