@@ -67,9 +67,8 @@ int ortho_fields(OrthoParams& p, const char* name, int type, int64_t batch, int6
   if (batch < 0 || rows < 0 || cols < 0 || rows > most || cols > most || type < 0 || type > 2 || steps < 1 ||
       steps > 64 || !(eps >= 0.0f))
     return fail(BLITZ_EINVAL, text);
-  if (rows > 0 && cols > 0 && batch > ((int64_t)1 << 38) / (((rows + 127) / 128 * 128) * ((cols + 127) / 128 * 128)))
-    return fail(BLITZ_EINVAL, text);
   if (!ortho_coefficients_ok(a, b, c, steps)) {
+    char text[160];
     snprintf(text, sizeof(text), "%s: coefficients let the iterates grow beyond 1.85 or the polynomial beyond 7.8", name);
     return fail(BLITZ_EINVAL, text);
   }
@@ -80,6 +79,11 @@ int ortho_fields(OrthoParams& p, const char* name, int type, int64_t batch, int6
   p.m = tall ? rows : cols;
   p.si = tall ? 1 : cols;
   p.sj = tall ? cols : 1;
+  // grids and tile numbers in 32 bits
+  const int64_t tiles = ((rows + 127) / 128) * ((cols + 127) / 128);
+  if (rows > 0 && cols > 0 &&
+      batch > (ortho_small_fits(p) || ortho_resident_fits(p) ? (int64_t)1 << 31 : ((int64_t)1 << 24) / tiles))
+    return fail(BLITZ_EINVAL, text);
   p.steps = steps;
   p.a = a;
   p.b = b;

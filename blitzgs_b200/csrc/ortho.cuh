@@ -17,7 +17,8 @@ __device__ __forceinline__ void ortho_scaling(double norm, float eps, float& up,
   int e = norm > 0.0 && norm <= 1e300 ? 14 - (ilogb(norm) + 1) : 0;
   e = max(-126, min(120, e));
   up = ldexpf(1.0f, e);
-  alpha = (float)(1.0 / ((norm + (double)eps) * ldexp(1.0, e)));
+  // zeros stay zeros, whatever eps is
+  alpha = norm == 0.0 ? 0.0f : (float)(1.0 / ((norm + (double)eps) * ldexp(1.0, e)));
 }
 
 // whether u needs two f16 terms, and how many steps use two

@@ -1049,6 +1049,8 @@ def _adam8(param, grad, m_codes, m_scales, r_codes, r_scales, visible, rows, n, 
     for c, s in ((m_codes, m_scales), (r_codes, r_scales)):
         if _code_rows(c, s, group, what) != (N, M, 1):
             raise RuntimeError(f"{what} needs float8_e4m3fn moments [{N}, {M}]")
+    if n == 0:
+        return
     if not grad.is_contiguous():
         grad = grad.contiguous()
     s, s_ptr = _seed(seed, param.device)
@@ -1136,13 +1138,13 @@ def orthogonal_update(param, grad, momentum, lr, *, beta=0.95, nesterov=True, we
     for t in (param, momentum):
         if t.dtype != torch.float32 or not t.is_contiguous() or t.shape != param.shape:
             raise RuntimeError("orthogonal_update needs contiguous float32 param and momentum of one shape")
-    if grad.dtype not in _VALUE_TYPES or grad.shape != param.shape:
-        raise RuntimeError("orthogonal_update needs a gradient of the parameter's shape, of 32 or 16 bits")
+    if grad.dtype not in _VALUE_TYPES or grad.shape != param.shape or grad.layout != torch.strided:
+        raise RuntimeError("orthogonal_update needs a dense gradient of the parameter's shape, of 32 or 16 bits")
     batch, rows, cols = _matrices(param, "orthogonal_update")
-    if batch and (param.data_ptr() == momentum.data_ptr() or grad.data_ptr() in (param.data_ptr(),
-                                                                                 momentum.data_ptr())):
-        raise RuntimeError("orthogonal_update needs param, grad and momentum in different memory")
     grad = grad.contiguous()
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in (param, momentum, grad))
+    if batch and (spans[0][1] > spans[1][0] or spans[1][1] > spans[2][0]):
+        raise RuntimeError("orthogonal_update needs param, grad and momentum in different memory")
     if scale is None:
         scale = math.sqrt(max(1.0, rows / cols)) if cols else 1.0
     ws, need = _ortho_workspace(batch, rows, cols, param.device)

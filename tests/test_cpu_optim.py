@@ -76,7 +76,7 @@ def test_orthogonalisation_entries_check_their_arguments():
         _rejects("blitz_orthogonal_update", ptr, ptr, type, ptr, batch, rows, cols, steps, *co, eps, 0.95, 0.05, 1, 1.0,
                  0.1, ws, size, None, **kw)
 
-    for sizes in ((-1, 4, 4), (1, -4, 4), (1, 4, 40000), (2 ** 40, 4, 4)):
+    for sizes in ((-1, 4, 4), (1, -4, 4), (1, 4, 40000), (2 ** 40, 4, 4), (2 ** 24, 200, 200)):
         both(*sizes, msg="bad sizes")
     for kw in (dict(steps=0), dict(steps=65), dict(type=3), dict(eps=-1.0), dict(eps=float("nan"))):
         both(1, 300, 300, **kw, msg="bad sizes")

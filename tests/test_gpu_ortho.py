@@ -134,6 +134,25 @@ def test_empty_and_strided(cuda_device):
         assert torch.equal(ops.orthogonalize(view), ops.orthogonalize(view.clone().contiguous()))
 
 
+@pytest.mark.parametrize("shape", [(3, 4), (9, 9), (60, 100), (150, 200)])
+def test_zeros_stay_zeros_without_eps(cuda_device, shape):
+    assert (ops.orthogonalize(torch.zeros(shape, device=cuda_device), eps=0.0) == 0).all()
+
+
+def test_more_small_matrices_than_a_grid_has_rows(cuda_device):
+    """20 million 1 x 2 matrices.  A vector has one singular value, |g| / (|g| + eps) at
+    first (eps shows in the shortest of so many), and the polynomial acts on it alone."""
+    g = torch.randn(20_000_000, 1, 2, device=cuda_device)
+    got = ops.orthogonalize(g).double().norm(dim=(1, 2))
+    norm = g.double().norm(dim=(1, 2))
+    s = norm / (norm + float(np.float32(1e-7)))
+    for _ in range(5):
+        a, b, c = (float(np.float32(v)) for v in ops.ORTHO_COEFFICIENTS)
+        s = s * (a + b * s ** 2 + c * s ** 4)
+    # 5 steps in 32 bits: each multiplies what came before by at most 3.45 and adds 6 roundings of 2^-24
+    assert (got - s).abs().max() <= 6 * 2.0 ** -24 * sum(3.45 ** k for k in range(5)) + 1e-6
+
+
 def test_a_repeated_call_gives_the_same_bits(cuda_device):
     for shape in ((15, 3), (50, 60), (300, 500), (4, 128, 256)):
         g = _input(shape, torch.float32).to(cuda_device)
@@ -224,6 +243,12 @@ def test_refusals(cuda_device):
     p, M = torch.zeros(5, 6, device=cuda_device), torch.zeros(5, 6, device=cuda_device)
     with pytest.raises(RuntimeError, match="different memory"):
         ops.orthogonal_update(p, g, p, 0.1)
+    flat = torch.zeros(60, device=cuda_device)
+    with pytest.raises(RuntimeError, match="different memory"):
+        ops.orthogonal_update(flat[:30].view(5, 6), g, flat[20:50].view(5, 6), 0.1)
+    ops.orthogonal_update(flat[:30].view(5, 6), g, flat[30:].view(5, 6), 0.1)
+    with pytest.raises(RuntimeError, match="dense"):
+        ops.orthogonal_update(p, g.to_sparse(), M, 0.1)
     with pytest.raises(RuntimeError, match="contiguous"):
         ops.orthogonal_update(p.t(), g.t(), M.t(), 0.1)
     with pytest.raises(RuntimeError, match="shape"):

@@ -275,6 +275,23 @@ def test_adam8_rows_outside_are_skipped(cuda_device):
     assert (m[1] > 0).flatten().nonzero().flatten().tolist() == [2, 8]
 
 
+def test_adam8_with_nothing_to_update(cuda_device):
+    """An empty row list, a mask without a visible Gaussian, a scene without Gaussians."""
+    N, M = 7, 45
+    p = torch.randn(N, M, device=cuda_device)
+    before = p.clone()
+    m, r = _store(N, M, 45, "e4m3", cuda_device), _store(N, M, 45, "e4m3", cuda_device)
+    args = (0.1, 0.9, 0.999, 1e-15)
+    ops.adam8_update_rows(p, p[:0].clone(), *m, *r, torch.empty(0, dtype=torch.int64, device=cuda_device), *args, N, M,
+                          group=45, seed=1)
+    ops.adam8_update(p, torch.ones_like(p), *m, *r, torch.zeros(N, dtype=torch.bool, device=cuda_device), *args, N, M,
+                     group=45, seed=1)
+    assert torch.equal(p, before) and (m[1] == 0).all() and (r[1] == 0).all()
+    m, r = _store(0, M, 45, "e4m3", cuda_device), _store(0, M, 45, "e4m3", cuda_device)
+    ops.adam8_update(p[:0], p[:0].clone(), *m, *r, torch.zeros(0, dtype=torch.bool, device=cuda_device), *args, 0, M,
+                     group=45, seed=1)
+
+
 def test_adam8_in_a_captured_graph_takes_its_seed_from_the_device(cuda_device):
     """A seed tensor counted up between replays gives each its own dithering: the
     replayed steps equal eager ones with the same seeds."""
