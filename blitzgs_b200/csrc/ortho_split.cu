@@ -23,7 +23,7 @@
 // Tensor memory holds four accumulators. Where two terms are used each takes
 // one k of 64 (the low terms first) and is then added up in registers: the tensor cores'
 // additions drop the bits below the accumulator's last one, those here round. Over
-// 1024 columns that is the difference between an error of 4e-5 and of 3e-6.
+// 1024 columns that is the difference between an error of 4e-5 and of 2e-6.
 #include <algorithm>
 
 #include "ortho_grid.cuh"
