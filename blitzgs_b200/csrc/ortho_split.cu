@@ -25,6 +25,7 @@
 // additions drop the bits below the accumulator's last one, those here round. Over
 // 1024 columns that is the difference between an error of 4e-5 and of 2e-6.
 #include <algorithm>
+#include <atomic>
 
 #include "ortho_grid.cuh"
 
@@ -522,7 +523,7 @@ int configure(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, int blocks, cu
 template <int S>
 int clusters(int sms) {
   if (S == 1) return sms;
-  static int known[64] = {};  // by device; the same answer whoever asks first
+  static std::atomic<int> known[64] = {};  // by device; the same answer whoever asks first
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
   if (known[dev] == 0) {

@@ -17,7 +17,7 @@ import numpy as np
 import pytest
 import torch
 
-from blitzgs_b200 import ops
+from blitzgs_b200 import _lib, ops
 from oracle import optim_oracle as O
 
 pytestmark = pytest.mark.gpu
@@ -132,6 +132,19 @@ def test_empty_and_strided(cuda_device):
     g = _input((90, 160), torch.float32).to(cuda_device)
     for view in (g.t(), g[3:80, 5:150], g[::2, ::3], g[:, :1].expand(90, 160)[:, 1:]):
         assert torch.equal(ops.orthogonalize(view), ops.orthogonalize(view.clone().contiguous()))
+
+
+@pytest.mark.parametrize("shape", [(500, 15, 3), (7, 9, 9), (5, 60, 100), (2, 150, 200)])
+def test_entry_in_place_and_with_a_dirty_workspace(cuda_device, shape):
+    """The C entry with out = g, and scratch full of NaN."""
+    g = _input(shape, torch.float32).to(cuda_device)
+    want = ops.orthogonalize(g)
+    need = _lib.load().blitz_orthogonalize_workspace_bytes(*shape)
+    ws = torch.full((need // 4 + 64,), float("nan"), device=cuda_device)
+    _lib.call("blitz_orthogonalize", g.data_ptr(), 0, g.data_ptr(), *shape, 5, *ops.ORTHO_COEFFICIENTS, 1e-7,
+              ws.data_ptr(), need, _lib.stream_ptr())
+    torch.cuda.synchronize()
+    assert torch.equal(g, want) and ws[need // 4:].isnan().all()
 
 
 @pytest.mark.parametrize("shape", [(3, 4), (9, 9), (60, 100), (150, 200)])
