@@ -64,20 +64,22 @@ struct Product {
 
 __device__ __forceinline__ void issue(const Product& q, uint32_t on, uint32_t d, uint32_t bar) {
   const uint32_t idesc = instruction_desc(q.n, q.b_mn);
+  // 16 of k further, in units of 16 bytes: 32 bytes along a row and after four of those the next
+  // 64 columns, or 16 rows
+  const uint32_t b_step = q.b_mn ? 128 : 2, b_four = q.b_mn ? 512 : kGroup >> 4;
   uint32_t add = 0;
+#pragma unroll
   for (int t = 0; t < 3; ++t) {
     // low * high, high * low, high * high
     if (t == 0 && !q.two_a || t == 1 && !q.two_b) continue;
-    const uint32_t a0 = smem_desc(q.a + (t == 0 ? q.a_term : 0), 16);
-    const uint32_t b0 = smem_desc(q.b + (t == 1 ? q.b_term : 0), q.b_mn ? kGroup : 16);
-    // 16 of k further, in units of 16 bytes: 32 bytes along a row, the next 64 columns after
-    // four of them, or 16 rows
-#pragma unroll 4
-    for (int k = 0; k < q.k; ++k) {
-      const uint32_t along = (uint32_t)(k >> 2) * (kGroup >> 4) + (uint32_t)(k & 3) * 2;
-      mma(on, d, a0 + along, b0 + (q.b_mn ? (uint32_t)k * 128 : along), idesc, add);
-      add = 1;
+    uint32_t a = smem_desc(q.a + (t == 0 ? q.a_term : 0), 16);
+    uint32_t b = smem_desc(q.b + (t == 1 ? q.b_term : 0), q.b_mn ? kGroup : 16);
+    int k = q.k;
+    for (; k >= 4; k -= 4, a += kGroup >> 4, b += b_four) {
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk, add = 1) mma(on, d, a + 2 * kk, b + b_step * kk, idesc, add);
     }
+    for (; k > 0; --k, a += 2, b += b_step, add = 1) mma(on, d, a, b, idesc, add);
   }
   mma_commit(on, bar);
 }
