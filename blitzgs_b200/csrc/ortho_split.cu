@@ -9,16 +9,15 @@
 // peer's shared memory came to 12 bytes a cycle, 5500 cycles a tile.)  Order of the sum: by
 // block, so the result does not depend on timing.
 //
-// Where there are tiles enough (S = 1), shared memory bounds the products: one of 128 x 128 x
-// 16 reads 8 KB of operands in 64 cycles' work and takes 85.  (Tiles of 128 x 256, 12 KB
-// in 128 cycles, have fewer units in flight and leave more SMs without one: 4260 us for 3760
-// at 4096^2. Pairs of blocks on 256 x 128 took 5530.)
+// Where there are tiles enough (S = 1) a k of 64 takes 760 cycles, the products' own rate; 2048^2 in
+// 32 bits takes 480 us, 4096^2 3.9 ms.  (Tiles of 128 x 256 have fewer units in flight and leave
+// more SMs without one: 4260 us for 3760 at 4096^2. Pairs of blocks on 256 x 128 took 5530.)
 //
 // The operands' ring holds the low terms of a k of 64 and the high ones as units of their own:
 // the low ones are free after two thirds of the products.  Two warps issue copies, every
 // second unit each, and two issue products, every second k of 64 each into accumulators of its
 // own: a wait that is already over still takes 125 cycles, a product's issue 45 and a copy's
-// 100, which one warp each would not hide behind 768 cycles of products.
+// 100; one warp each took 1350 cycles a k of 64.
 //
 // Tensor memory holds four accumulators. Where two terms are used each takes
 // one k of 64 (the low terms first) and is then added up in registers: the tensor cores'
