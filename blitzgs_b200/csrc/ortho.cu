@@ -12,10 +12,9 @@
 // steps by 485: rounding X to f16 once a step would leave the direction 1e-3
 // to 1e-2 off.  So X, A and B are kept as two f16 terms (high + low, 22 bits)
 // and a product is high*high + high*low + low*high, which leaves about 4e-6.
-// bf16 terms would need three for that.  Where the result is rounded to bf16
-// (off by 1.7e-3 itself) the last two steps, whose errors are hardly
-// multiplied any more, use the high terms alone; 16-bit inputs are exact in one
-// term, so step 0 reads one.  Everything is scaled by powers of two into
+// bf16 terms would need three for that.  16-bit inputs are exact in one term, so step 0
+// reads one of X; every other operand has two, whatever type the result is rounded to.
+// Everything is scaled by powers of two into
 // f16's range: |X_ij| <= 1.9 by 2^14, |A_ij| <= 3.7 by 2^14, |B_ij| < 7.9 by 2^13
 // (the caller's coefficients are checked to keep to that).
 //
@@ -235,7 +234,6 @@ int launch_ortho(const OrthoParams& o, void* workspace, cudaStream_t st) {
   p.ldm = q.ldm;
   p.ldn = q.ldn;
   p.two_in = ortho_two_in(o);
-  p.two_steps = ortho_two_steps(o);
   p.four = ortho_by_four(o);
   for (int i = 0; i < 2; ++i)
     if (int rc = make_map(&p.map_x[i], p.x[i], o.m, o.n, q.ldm, o.batch)) return rc;

@@ -21,11 +21,8 @@ __device__ __forceinline__ void ortho_scaling(double norm, float eps, float& up,
   alpha = norm == 0.0 ? 0.0f : (float)(1.0 / ((norm + (double)eps) * ldexp(1.0, e)));
 }
 
-// whether u needs two f16 terms, and how many steps use two
+// whether u needs two f16 terms
 __host__ __device__ inline bool ortho_two_in(const OrthoParams& p) { return p.param || p.g_type == kValueF32; }
-__host__ __device__ inline int ortho_two_steps(const OrthoParams& p) {
-  return !p.param && p.g_type == kValueBf16 ? (p.steps > 2 ? p.steps - 2 : 0) : p.steps;
-}
 
 // 32 bytes of global memory, a whole sector, by one lane
 __device__ __forceinline__ void store32(void* p, const uint32_t (&v)[8]) {

@@ -23,28 +23,24 @@ struct OrthoGrid {
   int n_parts;
   int ldm, ldn;
   int two_in;             // u needs two terms
-  int two_steps;          // steps 0 .. two_steps - 1 use two terms
   int four;               // ortho_by_four
 };
 
 enum OrthoPhase : int { kGram, kPoly, kApply };
 
-// which terms a phase reads and writes
+// which terms a phase reads
 struct OrthoTerms {
   int which, step;
-  bool two, two_a, two_b, write_two, last;
+  bool two_a, two_b, last;
   const CUtensorMap *ma, *mb;
 };
 __device__ __forceinline__ OrthoTerms ortho_terms(const OrthoGrid& p, int ph) {
   OrthoTerms t;
   t.step = ph / 3;
   t.which = ph - 3 * t.step;
-  t.two = t.step < p.two_steps;
-  const bool two_x = t.two && (t.step > 0 || p.two_in);
-  t.two_a = t.which == kGram ? two_x : t.two;
-  t.two_b = t.which == kPoly ? t.two : two_x;
-  // A and B are read by this step's own products, the new X by the next one's
-  t.write_two = t.which == kApply ? t.step + 1 < p.two_steps : t.two;
+  const bool two_x = t.step > 0 || p.two_in;
+  t.two_a = t.which == kGram ? two_x : true;
+  t.two_b = t.which == kPoly ? true : two_x;
   t.last = t.step == p.o.steps - 1 && t.which == kApply;
   t.ma = t.which == kGram ? &p.map_x[t.step & 1] : t.which == kPoly ? &p.map_a : &p.map_b;
   t.mb = t.which == kPoly ? &p.map_a : &p.map_x[t.step & 1];

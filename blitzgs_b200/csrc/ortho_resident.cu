@@ -114,7 +114,6 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) resident_kernel(OrthoP
   const Layout l = layout_of(n, m);
   uint8_t* A = X + 2 * l.x_term;
   const uint32_t xs = smem_addr(X), as = smem_addr(A), bar = smem_addr(&bar_mem);
-  const int two_steps = ortho_two_steps(p);
   const bool two_in = ortho_two_in(p), wide = p.sj == 1;
   if (tid == 0) {
     dead_flag = 0;
@@ -201,7 +200,7 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) resident_kernel(OrthoP
 
 #pragma unroll 1
     for (int s = 0; s < p.steps; ++s) {
-      const bool two = s < two_steps, two_x = two && (s > 0 || two_in), two_next = s + 1 < two_steps;
+      const bool two_x = s > 0 || two_in;
       const bool last = s + 1 == p.steps;
       const float fx = s == 0 ? alpha : 1.0f / kScaleX;
 #pragma unroll 1
@@ -213,8 +212,8 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) resident_kernel(OrthoP
           q.b = which == 1 ? as : xs;
           q.a_term = which == 0 ? l.x_term : l.a_term;
           q.b_term = which == 1 ? l.a_term : l.x_term;
-          q.two_a = which == 0 ? two_x : two;
-          q.two_b = which == 1 ? two : two_x;
+          q.two_a = which == 0 ? two_x : true;
+          q.two_b = which == 1 ? true : two_x;
           q.k = (which == 0 ? l.mp : l.np) / 16;
           q.n = which == 2 ? l.mp : l.np;
           q.b_mn = which == 2;
@@ -247,7 +246,6 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) resident_kernel(OrthoP
             continue;
           }
           // columns past np / mp hold what was left there; nothing reads their terms
-          const bool two_out = which == 2 ? two_next : two;
           uint8_t* dst = which == 2 ? X : A;
           const int term = which == 2 ? l.x_term : l.a_term;
           const float f = which == 0 ? fx * fx * kScaleA : which == 1 ? p.c * (kScaleB / (kScaleA * kScaleA))
@@ -258,9 +256,7 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) resident_kernel(OrthoP
             const int at = chunk_at(row, c + k);
             if (which == 1) {
               // B = a I + b A + c A^2 in A's place: this thread alone reads and writes here
-              const uint4 h4 = *(const uint4*)(dst + at);
-              uint4 l4 = make_uint4(0, 0, 0, 0);
-              if (two) l4 = *(const uint4*)(dst + term + at);
+              const uint4 h4 = *(const uint4*)(dst + at), l4 = *(const uint4*)(dst + term + at);
               const uint32_t hs[4] = {h4.x, h4.y, h4.z, h4.w}, ls[4] = {l4.x, l4.y, l4.z, l4.w};
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
@@ -280,7 +276,7 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) resident_kernel(OrthoP
             uint4 hi, lo;
             split8(v + k, hi, lo);
             *(uint4*)(dst + at) = hi;
-            if (two_out) *(uint4*)(dst + term + at) = lo;
+            *(uint4*)(dst + term + at) = lo;
           }
         }
         tcgen05_before_sync();

@@ -19,9 +19,8 @@
 // own: a wait that is already over still takes 125 cycles, a product's issue 45 and a copy's
 // 100; one warp each took 1350 cycles a k of 64.
 //
-// Tensor memory holds four accumulators. Where two terms are used each takes
-// one k of 64 (the low terms first) and is then added up in registers: the tensor cores'
-// additions drop the bits below the accumulator's last one, those here round. Over
+// Tensor memory holds four accumulators. Each takes one k of 64 (the low terms first) and
+// is then added up in registers: the tensor cores' additions drop the bits below the accumulator's last one, those here round. Over
 // 1024 columns that is the difference between an error of 4e-5 and of 2e-6.
 #include <algorithm>
 #include <atomic>
@@ -52,7 +51,6 @@ struct Shape {
   int mt, nt, per, total;  // per: tiles of one matrix
   int k0, boxes;           // this block's k, in boxes
   int units;               // units of a box: 2 where an operand has two terms
-  int accs;                // accumulators of a tile: one a box, or one for every second box
 };
 
 template <int S>
@@ -71,7 +69,6 @@ __device__ __forceinline__ Shape shape_of(const OrthoGrid& p, int ph, int rank) 
   s.k0 = S > 1 ? boxes * rank / S : 0;
   s.boxes = (S > 1 ? boxes * (rank + 1) / S : boxes) - s.k0;
   s.units = s.t.two_a || s.t.two_b ? 2 : 1;
-  s.accs = s.t.two ? s.boxes : min(s.boxes, 2);
   return s;
 }
 
@@ -103,20 +100,20 @@ __device__ __forceinline__ void load_a(const OrthoGrid& p, const OrthoTerms& t, 
     // rows are a whole number of 64 columns long, so 16 from one below n are in the row
     if (t.which == kPoly && col + 2 * k < n) {
       load32(A + 2 * k, *(uint32_t(*)[8])(hi + k));
-      if (t.two_a) load32(A + (int64_t)n * p.ldn + 2 * k, *(uint32_t(*)[8])(lo + k));
+      load32(A + (int64_t)n * p.ldn + 2 * k, *(uint32_t(*)[8])(lo + k));
     }
   }
 }
 
 // C values' terms to row `dst`, the low ones `low` further, as far as there are columns
 template <int C>
-__device__ __forceinline__ void store_terms(__half* dst, int64_t low, int left, bool two, const uint32_t (&h)[C / 2],
+__device__ __forceinline__ void store_terms(__half* dst, int64_t low, int left, const uint32_t (&h)[C / 2],
                                             const uint32_t (&l)[C / 2]) {
 #pragma unroll
   for (int k = 0; k < C / 2; k += 8) {
     if (2 * k >= left) break;
     store32(dst + 2 * k, *(const uint32_t(*)[8])(h + k));
-    if (two) store32(dst + low + 2 * k, *(const uint32_t(*)[8])(l + k));
+    store32(dst + low + 2 * k, *(const uint32_t(*)[8])(l + k));
   }
 }
 
@@ -137,7 +134,7 @@ __device__ __forceinline__ void finish(const OrthoGrid& p, const OrthoTerms& t, 
 #pragma unroll
       for (int k = 0; k < C / 2; ++k) h[k] = split2(v[2 * k], v[2 * k + 1], l[k]);
       store_terms<C>(p.x[(t.step + 1) & 1] + ((int64_t)(2 * b) * n + row) * p.ldm + col, (int64_t)n * p.ldm, m - col,
-                     t.write_two, h, l);
+                     h, l);
       return;
     }
     const int64_t at = (int64_t)b * n * m + row * p.o.si;
@@ -204,7 +201,7 @@ __device__ __forceinline__ void finish(const OrthoGrid& p, const OrthoTerms& t, 
   uint32_t h[C / 2], l[C / 2];
 #pragma unroll
   for (int k = 0; k < C / 2; ++k) h[k] = split2(v[2 * k], v[2 * k + 1], l[k]);
-  if (row < n) store_terms<C>(out + (int64_t)row * p.ldn + col, low, n - col, t.write_two, h, l);
+  if (row < n) store_terms<C>(out + (int64_t)row * p.ldn + col, low, n - col, h, l);
   if (!mirror) return;
   // the mirror image: neighbouring lanes (rows) swap halves, so that each writes two
   // rows' values of one column in one word
@@ -219,7 +216,7 @@ __device__ __forceinline__ void finish(const OrthoGrid& p, const OrthoTerms& t, 
     // ldn is even, so a pair that begins below n stays inside its row
     if (even < n) {
       *(uint32_t*)(to + (int64_t)(2 * k) * p.ldn) = hw;
-      if (t.write_two) *(uint32_t*)(to + (int64_t)(2 * k) * p.ldn + low) = lw;
+      *(uint32_t*)(to + (int64_t)(2 * k) * p.ldn + low) = lw;
     }
   }
 }
@@ -267,9 +264,10 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
   constexpr uint32_t tmem = 0;
   const uint32_t on = elected();
 
-  // Units and accumulators are numbered through the whole run, by every role alike: number u
-  // lies in slot u % kUnits and is that slot's use u / kUnits, whose parity is waited for.
-  uint32_t unit0 = 0, acc0 = 0, box0 = 0, ph_xf = 0, ph_xe = 1;
+  // Units and boxes are numbered through the whole run, by every role alike: unit u lies in
+  // slot u % kUnits and is that slot's use u / kUnits, whose parity is waited for; box a has
+  // accumulator a % kAccs.
+  uint32_t unit0 = 0, box0 = 0, ph_xf = 0, ph_xe = 1;
   unsigned arrivals = 0;
   bool alive = true;
   const int phases = 3 * p.o.steps;
@@ -314,17 +312,13 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
       // when the other has what it waited for before it: a parity cannot tell a barrier two
       // uses behind from one that is ready.
       const uint32_t mine = warp - 2;
-      uint32_t u0 = unit0, a0 = acc0, g0 = box0;
-      for (int t = 0; t < tiles && !*dead; ++t, u0 += s.boxes * s.units, a0 += s.accs, g0 += s.boxes) {
-        uint32_t add = 0;
+      uint32_t u0 = unit0, g0 = box0;
+      for (int t = 0; t < tiles && !*dead; ++t, u0 += s.boxes * s.units, g0 += s.boxes) {
         for (int k = (int)((mine ^ g0) & 1); k < s.boxes; k += 2) {
-          const uint32_t turn = (g0 + k) >> 1;
+          const uint32_t a = g0 + k, turn = a >> 1, d = tmem + a % kAccs * kB;
           if (!mbar_wait(token + 8 * mine, (turn + (mine ? 0 : 1)) & 1, dead)) break;
-          const uint32_t a = a0 + (s.t.two ? k : k & 1), d = tmem + a % kAccs * kB;
-          if (s.t.two || k < 2) {
-            if (!mbar_wait(acc_empty + 8 * (a % kAccs), (a / kAccs & 1) ^ 1, dead)) break;
-            add = 0;
-          }
+          uint32_t add = 0;
+          if (!mbar_wait(acc_empty + 8 * (a % kAccs), (a / kAccs & 1) ^ 1, dead)) break;
           const uint32_t ul = u0 + k * s.units, uh = ul + s.units - 1;
           const uint32_t lo = ul % kUnits<S>, hi = uh % kUnits<S>;
           if (s.units == 2 && !mbar_wait(full + 8 * lo, ul / kUnits<S> & 1, dead)) break;
@@ -351,11 +345,11 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
 #pragma unroll
           for (int kk = 0; kk < kBK / 16; ++kk, add = 1) mma(on, d, ah + 2 * kk, bh + b_step * kk, idesc, add);
           mma_commit(on, empty + 8 * hi);
-          if (s.t.two || k + 2 >= s.boxes) mma_commit(on, acc_full + 8 * (a % kAccs));
+          mma_commit(on, acc_full + 8 * (a % kAccs));
         }
       }
     } else {
-      uint32_t a = acc0;
+      uint32_t a = box0;
       // a block finishes W columns of a tile, a thread C of them in one row: the first or
       // second half.  It adds up that half of every block's columns.
       constexpr int W = kB / S, C = W / 2;
@@ -372,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
 #pragma unroll
         for (int i = 0; i < 64; ++i) acc[i] = 0.0f;
         bool ok = true;
-        for (int j = 0; j < s.accs; ++j, ++a) {
+        for (int j = 0; j < s.boxes; ++j, ++a) {
           const uint32_t ac = a % kAccs;
           ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * ac, a / kAccs & 1, dead)) && ok;
           tcgen05_after_sync();
@@ -475,7 +469,6 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
     __syncwarp();
     unit0 += (uint32_t)(tiles * s.boxes * s.units);
     box0 += (uint32_t)(tiles * s.boxes);
-    acc0 += (uint32_t)(tiles * s.accs);
     if (ph + 1 < phases) {
       arrivals += gridDim.x;
       alive = ortho_barrier(p.barrier, arrivals, dead);

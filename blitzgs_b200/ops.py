@@ -1105,9 +1105,8 @@ def _ortho_workspace(batch, rows, cols, device):
 def orthogonalize(g, *, steps=5, coefficients=ORTHO_COEFFICIENTS, eps=1e-7):
     """The direction of each matrix of g [..., rows, cols] (float32, bfloat16
     or float16): its singular values driven towards 1 by ``steps`` Newton-Schulz
-    steps (blitz_orthogonalize).  Returns a new tensor of g's type.  float32
-    and float16 results are within about 1e-5 (2-norm) of the formula before
-    their rounding, bfloat16 ones within about 2e-3."""
+    steps (blitz_orthogonalize).  Returns a new tensor of g's type, within
+    about 1e-5 (2-norm) of the formula before its rounding to that type."""
     _same_device(g)
     if g.dtype not in _VALUE_TYPES:
         raise RuntimeError(f"orthogonalize: values are of 32 or 16 bits, got {g.dtype}")
