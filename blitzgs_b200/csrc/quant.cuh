@@ -108,11 +108,12 @@ __device__ __forceinline__ uint8_t encode(float x, const GroupCode<KIND>& g, uin
   }
 }
 
+// two codes -> their values.  The e4m3 bytes 0x7f and 0xff, which encode never makes but a
+// caller's tensor may hold, are NaN in the format and here.
 template <int KIND>
-__device__ __forceinline__ float decode(uint8_t c, float s) {
-  if (KIND == kInt8) return __fmul_rn((float)(int8_t)c, s);
-  const uint32_t bits = ((uint32_t)c & 0x7fu) << 20 | ((uint32_t)c & 0x80u) << 24;
-  return __fmul_rn(__fmul_rn(__int_as_float((int)bits), 0x1p120f), s);
+__device__ __forceinline__ float2 decode2(uint8_t x, uint8_t y, float s) {
+  const float2 v = KIND == kInt8 ? make_float2((float)(int8_t)x, (float)(int8_t)y) : e4m3_pair(x, y);
+  return make_float2(__fmul_rn(v.x, s), __fmul_rn(v.y, s));
 }
 
 __device__ __forceinline__ float to_float(float x) { return x; }

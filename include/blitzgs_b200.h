@@ -531,7 +531,8 @@ int blitz_adam_update_rows(float* param, const float* grad_rows, float* exp_avg,
  *   kind 1, e4m3: scale = the smallest power of two (>= 2^-126) with
  *     max|x| / scale <= 448 (0 for a group of zeros), code = x / scale rounded
  *     to e4m3; storing values read from such a store changes nothing.
- * A group with a NaN or an infinity gets a NaN scale and reads back as NaN.
+ * A group with a NaN or an infinity gets a NaN scale and reads back as NaN; so
+ * does an e4m3 code that is NaN in that format, should a caller's store hold one.
  * value_type: 0 float, 1 bf16, 2 fp16.
  *
  * write stores values (row j value_stride elements after row j - 1) at row
