@@ -101,6 +101,9 @@ int ortho_start(const OrthoParams& p, const char* name, void* workspace, size_t 
   return check(launch_ortho(p, workspace, S(stream)), name);
 }
 
+// values of a row held in 8 bits: columns are counted in 32 bits
+constexpr int64_t kMaxRow = (int64_t)1 << 30;
+
 // 32 lanes a (row, group) at most, 256 threads a block, 2^31 - 1 blocks
 inline bool too_many_units(int64_t n, int64_t D, int group) {
   const int64_t G = (D + group - 1) / group, most = ((int64_t)1 << 31) * 8 - 8;
@@ -110,7 +113,7 @@ inline bool too_many_units(int64_t n, int64_t D, int group) {
 // the checks and fields that the row store's write and read share
 int quant_sizes(QuantParams& q, int kind, const int64_t* rows, int64_t n, int64_t N, int64_t D, int group,
                 const char* what) {
-  if (n < 0 || N < 0 || D < 0 || D > ((int64_t)1 << 30) || group < 1 || group > 256 || kind < 0 || kind > 1 ||
+  if (n < 0 || N < 0 || D < 0 || D > kMaxRow || group < 1 || group > 256 || kind < 0 || kind > 1 ||
       q.type < 0 || q.type > 2 || (!rows && n > N) || too_many_units(n, D, group))
     return fail(BLITZ_EINVAL, what);
   q.kind = kind;
@@ -722,7 +725,7 @@ int blitz_adam8_update(float* param, const float* grad, void* m_codes, float* m_
                        float* r_scales, const uint8_t* visible, const int64_t* rows, int64_t n_rows, float grad_scale,
                        float lr, float b1, float one_minus_b1, float b2, float one_minus_b2, float eps, int64_t N,
                        int64_t M, int group, uint32_t seed, const int64_t* seed_ptr, void* stream) {
-  if (N < 0 || M <= 0 || n_rows < 0 || group < 1 || group > 256 || too_many_units(rows ? n_rows : N, M, group))
+  if (N < 0 || M <= 0 || M > kMaxRow || n_rows < 0 || group < 1 || group > 256 || too_many_units(rows ? n_rows : N, M, group))
     return fail(BLITZ_EINVAL, "blitz_adam8_update: bad sizes");
   if ((visible != nullptr) == (rows != nullptr) && (rows || N > 0))
     return fail(BLITZ_EINVAL, "blitz_adam8_update: give either visible or rows");

@@ -526,7 +526,7 @@ int blitz_adam_update_rows(float* param, const float* grad_rows, float* exp_avg,
 /*
  * Rows of values held in 8 bits (no reference counterpart: the reference
  * keeps every optimizer state in 32 bits).  codes [N, D] and scales [N, G],
- * G = ceil(D / group), group 1..256: value = code * scale of its group.
+ * G = ceil(D / group), D <= 2^30, group 1..256: value = code * scale of its group.
  *   kind 0, int8: scale = max|x| / 127, code = x / scale rounded;
  *   kind 1, e4m3: scale = the smallest power of two (>= 2^-126) with
  *     max|x| / scale <= 448 (0 for a group of zeros), code = x / scale rounded
@@ -560,7 +560,7 @@ int blitz_quant_rows_read(const void* codes, const float* scales, int kind, cons
  * blitz_quant_rows_write (r with seed ^ 0x5BF03635, and never to zero where
  * it is positive).  Give either visible (uint8 [N], grad [N, M]) or
  * rows (int64 [n_rows], distinct, grad [n_rows, M]); rows outside [0, N) are
- * skipped, and the other Gaussians keep their parameter and state.
+ * skipped, and the other Gaussians keep their parameter and state.  M <= 2^30.
  */
 int blitz_adam8_update(float* param, const float* grad, void* m_codes, float* m_scales, void* r_codes,
                        float* r_scales, const uint8_t* visible, const int64_t* rows, int64_t n_rows, float grad_scale,
