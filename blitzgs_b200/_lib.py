@@ -52,6 +52,7 @@ SIGNATURES = {
                                       _vp]),
     "blitz_quant_rows_read": (_i32, [_vp, _vp, _i32, _vp, _i64, _i64, _i64, _i32, _vp, _i32, _vp]),
     "blitz_adam8_update": (_i32, [_vp] * 8 + [_i64] + [_f32] * 7 + [_i64, _i64, _i32, _i32, _vp, _vp]),
+    "blitz_orthogonalize_wait_limit": (_i64, [_i64]),
     "blitz_orthogonalize_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "blitz_orthogonalize": (_i32, [_vp, _i32, _vp, _i64, _i64, _i64, _i32, _f32, _f32, _f32, _f32, _vp, _sz, _vp]),
     "blitz_orthogonal_update": (_i32, [_vp, _vp, _i32, _vp, _i64, _i64, _i64, _i32] + [_f32] * 6 + [_i32, _f32, _f32,

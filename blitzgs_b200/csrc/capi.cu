@@ -1,4 +1,5 @@
 // extern "C" entry points (declared in include/blitzgs_b200.h).
+#include <atomic>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
@@ -29,6 +30,8 @@ int fail(int code, const char* what) {
 int check(int code, const char* what) { return code == 0 ? 0 : fail(code, what); }
 
 inline cudaStream_t S(void* s) { return reinterpret_cast<cudaStream_t>(s); }
+
+std::atomic<long long> ortho_wait_limit{kOrthoWaitLimit};
 
 // Whether the iterates stay inside what the kernels' scaled f16 terms hold:
 // singular values s in [0, 1] under s <- s (a + b s^2 + c s^4), largest values
@@ -89,6 +92,7 @@ int ortho_fields(OrthoParams& p, const char* name, int type, int64_t batch, int6
   p.b = b;
   p.c = c;
   p.eps = eps;
+  p.wait_limit = ortho_wait_limit.load(std::memory_order_relaxed);
   return 0;
 }
 
@@ -756,6 +760,10 @@ int blitz_adam8_update(float* param, const float* grad, void* m_codes, float* m_
   a.seed = seed;
   a.seed_ptr = seed_ptr;
   return check(launch_adam8(a, S(stream)), "blitz_adam8_update");
+}
+
+int64_t blitz_orthogonalize_wait_limit(int64_t cycles) {
+  return cycles < 0 ? ortho_wait_limit.load() : ortho_wait_limit.exchange(cycles);
 }
 
 size_t blitz_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols) {

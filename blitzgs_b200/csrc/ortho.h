@@ -21,7 +21,11 @@ struct OrthoParams {
   float beta, one_minus_beta;
   int nesterov;
   float keep, alpha;  // param = param * keep - alpha * direction
+  long long wait_limit;  // cycles after which a wait within a kernel gives up
 };
+
+// about two seconds of the SM's clock
+constexpr long long kOrthoWaitLimit = 4000000000ll;
 
 size_t ortho_workspace_bytes(const OrthoParams& p);
 int launch_ortho(const OrthoParams& p, void* workspace, cudaStream_t st);

@@ -48,7 +48,7 @@ __device__ __forceinline__ OrthoTerms ortho_terms(const OrthoGrid& p, int ph) {
 }
 
 // every block of the grid has arrived, and what each wrote (for its reads and its copies) is seen
-__device__ __forceinline__ bool ortho_barrier(unsigned* counter, unsigned target, volatile int* dead) {
+__device__ __forceinline__ bool ortho_barrier(unsigned* counter, unsigned target, volatile int* dead, long long limit) {
   fence_async_global();
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -58,7 +58,7 @@ __device__ __forceinline__ bool ortho_barrier(unsigned* counter, unsigned target
       unsigned seen;
       asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(counter) : "memory");
       if (seen >= target) break;
-      if (*dead || clock64() - t0 > kGiveUp || ((volatile unsigned*)counter)[1]) {
+      if (*dead || clock64() - t0 > limit || ((volatile unsigned*)counter)[1]) {
         *dead = 1;
         break;
       }

@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) resident_kernel(OrthoP
           q.b_mn = which == 2;
           issue(q, on, tmem, bar);
         }
-        mbar_wait(bar, parity, dead);
+        mbar_wait(bar, parity, dead, p.wait_limit);
         parity ^= 1;
         tcgen05_after_sync();
         __syncwarp();

@@ -263,6 +263,7 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
   // be the same for the whole warp)
   constexpr uint32_t tmem = 0;
   const uint32_t on = elected();
+  const long long limit = p.o.wait_limit;
 
   // Units and boxes are numbered through the whole run, by every role alike: unit u lies in
   // slot u % kUnits and is that slot's use u / kUnits, whose parity is waited for; box a has
@@ -277,15 +278,18 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
     const int tiles = first < s.total ? (s.total - first + by - 1) / by : 0;
     if (warp < 2) {
       uint32_t u = unit0;
-      for (int t = first; t < s.total && !*dead; t += by) {
+      bool go = true;  // until a wait gives up
+      for (int t = first; t < s.total && go; t += by) {
         int b, mi, ni;
         tile_of(s, t, b, mi, ni);
-        for (int k = s.k0; k < s.k0 + s.boxes; ++k) {
+        for (int k = s.k0; k < s.k0 + s.boxes && go; ++k) {
           // the low terms, then the high ones
           for (int term = s.units - 1; term >= 0; --term, ++u) {
             if ((u & 1) != (uint32_t)warp) continue;
             const uint32_t slot = u % kUnits<S>;
-            if (!mbar_wait(empty + 8 * slot, (u / kUnits<S> & 1) ^ 1, dead)) break;
+            // by lane: the one that copies goes on as long as its own waits end
+            go = mbar_wait(empty + 8 * slot, (u / kUnits<S> & 1) ^ 1, dead, limit);
+            if (!go) break;
             const bool has_a = term == 0 || s.t.two_a, has_b = term == 0 || s.t.two_b;
             const uint32_t bar = full + 8 * slot, dst = ring_addr + slot * kUnit;
             mbar_expect(on, bar, (has_a ? 2 * kBox : 0) + (has_b ? 2 * kBox : 0));
@@ -313,18 +317,20 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
       // uses behind from one that is ready.
       const uint32_t mine = warp - 2;
       uint32_t u0 = unit0, g0 = box0;
-      for (int t = 0; t < tiles && !*dead; ++t, u0 += s.boxes * s.units, g0 += s.boxes) {
+      bool go = true;  // until a wait gives up
+      for (int t = 0; t < tiles && go; ++t, u0 += s.boxes * s.units, g0 += s.boxes) {
         for (int k = (int)((mine ^ g0) & 1); k < s.boxes; k += 2) {
           const uint32_t a = g0 + k, turn = a >> 1, d = tmem + a % kAccs * kB;
-          if (!mbar_wait(token + 8 * mine, (turn + (mine ? 0 : 1)) & 1, dead)) break;
-          uint32_t add = 0;
-          if (!mbar_wait(acc_empty + 8 * (a % kAccs), (a / kAccs & 1) ^ 1, dead)) break;
           const uint32_t ul = u0 + k * s.units, uh = ul + s.units - 1;
           const uint32_t lo = ul % kUnits<S>, hi = uh % kUnits<S>;
-          if (s.units == 2 && !mbar_wait(full + 8 * lo, ul / kUnits<S> & 1, dead)) break;
-          if (!mbar_wait(full + 8 * hi, uh / kUnits<S> & 1, dead)) break;
-          if (lane == 0) mbar_arrive(token + 8 * (mine ^ 1));
-          __syncwarp();
+          go = mbar_wait(token + 8 * mine, (turn + (mine ? 0 : 1)) & 1, dead, limit) &&
+               mbar_wait(acc_empty + 8 * (a % kAccs), (a / kAccs & 1) ^ 1, dead, limit) &&
+               (s.units == 1 || mbar_wait(full + 8 * lo, ul / kUnits<S> & 1, dead, limit)) &&
+               mbar_wait(full + 8 * hi, uh / kUnits<S> & 1, dead, limit);
+          go = whole_warp(go);
+          if (!go) break;
+          uint32_t add = 0;
+          mbar_arrive(on, token + 8 * (mine ^ 1));
           tcgen05_after_sync();
           const uint32_t ah = smem_desc(ring_addr + hi * kUnit, 16),
                          bh = smem_desc(ring_addr + hi * kUnit + 2 * kBox, b_lead);
@@ -355,8 +361,9 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
       constexpr int W = kB / S, C = W / 2;
       const int quarter = warp & 3, half = (warp >> 2) - 1, local = quarter * 32 + lane;
       const uint32_t rows = tmem + ((uint32_t)(quarter * 32) << 16) + half * C;
-      // Warps that gave up go through the rest without waiting (and without arriving): they
+      // Warps that gave up go through the rest of the phase without arriving or sending: they
       // meet at a barrier of their own.
+      bool ok = true;
       for (int t = first; t < s.total; t += by) {
         int b, mi, ni;
         tile_of(s, t, b, mi, ni);
@@ -365,10 +372,9 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
         float acc[64];
 #pragma unroll
         for (int i = 0; i < 64; ++i) acc[i] = 0.0f;
-        bool ok = true;
         for (int j = 0; j < s.boxes; ++j, ++a) {
           const uint32_t ac = a % kAccs;
-          ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * ac, a / kAccs & 1, dead)) && ok;
+          ok = whole_warp(mbar_wait(acc_full + 8 * ac, a / kAccs & 1, dead, limit)) && ok;
           tcgen05_after_sync();
           if constexpr (S == 4) {
 #pragma unroll
@@ -389,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
           }
           tcgen05_before_sync();
           __syncwarp();
-          if (lane == 0 && ok) mbar_arrive(acc_empty + 8 * ac);
+          if (ok) mbar_arrive(on, acc_empty + 8 * ac);
         }
         if constexpr (S == 1) {
 #pragma unroll
@@ -406,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
           // the order of their ranks
           constexpr uint32_t kSlot = W * kB * 4;
           // what this block sent last has been read, so it has also left
-          ok = __all_sync(0xffffffffu, mbar_wait_cluster(x_empty, ph_xe, dead)) && ok;
+          ok = whole_warp(mbar_wait_cluster(x_empty, ph_xe, dead, limit)) && ok;
           ph_xe ^= 1;
           float4* out = (float4*)(ring + kRing<S>);
           float v[C];
@@ -437,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
               peer_copy(on, peer_addr(incoming + at * kSlot, to), exchange + slot * kSlot, kSlot, peer_addr(x_full, to));
             }
           }
-          ok = __all_sync(0xffffffffu, mbar_wait_cluster(x_full, ph_xf, dead)) && ok;
+          ok = whole_warp(mbar_wait_cluster(x_full, ph_xf, dead, limit)) && ok;
           ph_xf ^= 1;
           const float4* got = (const float4*)(ring + kRing<S> + kExchange<S>);
           float sum[C];
@@ -471,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
     box0 += (uint32_t)(tiles * s.boxes);
     if (ph + 1 < phases) {
       arrivals += gridDim.x;
-      alive = ortho_barrier(p.barrier, arrivals, dead);
+      alive = ortho_barrier(p.barrier, arrivals, dead, limit);
     }
   }
   __syncthreads();

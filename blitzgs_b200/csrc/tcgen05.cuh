@@ -2,7 +2,7 @@
 // and tensor copies (sm_100a), as the orthogonalisation kernels use them: one block (cta_group::1),
 // f16 operands in shared memory with 128-byte swizzle, 32-bit accumulators.
 //
-// Every wait on a barrier gives up after two seconds: it then sets the block's
+// Every wait on a barrier gives up after `limit` cycles: it then sets the block's
 // `dead` word, on which every other wait of the block gives up too.
 #pragma once
 #include <cuda.h>
@@ -16,8 +16,11 @@ __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+// by the lane of a whole warp that has `on`
+__device__ __forceinline__ void mbar_arrive(uint32_t on, uint32_t bar) {
+  asm volatile(
+      "{\n .reg .pred e;\n setp.ne.u32 e, %1, 0;\n @e mbarrier.arrive.shared::cta.b64 _, [%0];\n}" ::"r"(bar), "r"(on)
+      : "memory");
 }
 // 1 in one lane of a whole warp, always the same one
 __device__ __forceinline__ uint32_t elected() {
@@ -34,23 +37,24 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// cycles of this SM's clock: about two seconds (the global timer takes about a
-// microsecond to read, and most waits are shorter)
-constexpr long long kGiveUp = 4000000000ll;
-
-// false: gave up (or another thread of the block has)
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
+// false: gave up (or another thread of the block has).  The limit is in cycles of this SM's clock:
+// the global timer takes about a microsecond to read, and most waits are shorter.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* dead, long long limit) {
   if (mbar_try(bar, parity)) return true;
   const long long t0 = clock64();
   while (!mbar_try(bar, parity)) {
     if (*dead) return false;
-    if (clock64() - t0 > kGiveUp) {
+    if (clock64() - t0 > limit) {
       *dead = 1;
       return false;
     }
   }
   return true;
 }
+// The same answer for every lane of a whole warp: a wait can end for one lane in the moment
+// in which another gives up, and lanes that go different ways from there would wait for each
+// other for ever, one part at the warp's next barrier, the other at the block's.
+__device__ __forceinline__ bool whole_warp(bool waited) { return __all_sync(0xffffffffu, waited); }
 
 // by the lane of a whole warp that has `on`, as the products below
 __device__ __forceinline__ void tma_load(uint32_t on, uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
@@ -104,12 +108,12 @@ __device__ __forceinline__ bool mbar_try_cluster(uint32_t bar, uint32_t parity) 
       : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, volatile int* dead) {
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, volatile int* dead, long long limit) {
   if (mbar_try_cluster(bar, parity)) return true;
   const long long t0 = clock64();
   while (!mbar_try_cluster(bar, parity)) {
     if (*dead) return false;
-    if (clock64() - t0 > kGiveUp) {
+    if (clock64() - t0 > limit) {
       *dead = 1;
       return false;
     }

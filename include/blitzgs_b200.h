@@ -587,6 +587,10 @@ int blitz_adam8_update(float* param, const float* grad, void* m_codes, float* m_
  * needed), 256-byte aligned, any contents; calls that may run at the same
  * time need their own.
  */
+/* How many cycles of the SM's clock a wait within these kernels lasts before it
+ * gives up; sets it for the calls that follow (negative: no change) and
+ * returns what it was, at first 4e9 (about two seconds). */
+int64_t blitz_orthogonalize_wait_limit(int64_t cycles);
 size_t blitz_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols);
 int blitz_orthogonalize(const void* g, int value_type, void* out, int64_t batch, int64_t rows, int64_t cols, int steps,
                         float a, float b, float c, float eps, void* workspace, size_t workspace_bytes, void* stream);
