@@ -23,9 +23,13 @@
 // the whole grid. There `sum_kernel` advances the momentum and adds up squares (in 64 bits, in
 // a fixed order), `layout_kernel` writes X_0's terms, and one persistent cooperative
 // kernel runs all 3 * steps products with a grid-wide barrier between them, so a step
-// costs no launch.  In it one warp copies tiles of 64 columns by TMA (128-byte swizzle), one
-// warp issues the products, and eight warps move finished tiles out of tensor memory.  Every
-// wait gives up after two seconds: the outputs are then NaN.
+// costs no launch.  In it two warps copy tiles of 64 columns by TMA (128-byte swizzle), two
+// issue the products, and eight warps move finished tiles out of tensor memory.
+//
+// Every wait gives up after two seconds (see wait_limit).  In `resident_kernel` that block's matrix
+// is then NaN.  Over the grid the other blocks learn of it at the next barrier, and
+// `lost_kernel`, which runs when all of them have ended and so after all that they wrote, makes all
+// outputs of the call NaN.  (In a call of 127 us its launch does not show.)
 #include <algorithm>
 
 #include "ortho_grid.cuh"
@@ -41,7 +45,7 @@ constexpr int kMaxParts = 256;
 template <class T, bool UPDATE, int V>
 __global__ void __launch_bounds__(256) sum_kernel(OrthoParams o, double* parts, unsigned* barrier, int n_parts) {
   __shared__ double sums[8];
-  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 2) barrier[threadIdx.x] = 0u;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *barrier = 0u;
   const int size = (int)(o.n * o.m), per = ((size + n_parts - 1) / n_parts + 3) / 4 * 4;
   for (int64_t b = blockIdx.y; b < o.batch; b += gridDim.y) {
     const int lo = (int)min((int64_t)size, (int64_t)blockIdx.x * per), hi = (int)min((int64_t)size, (int64_t)lo + per);
@@ -147,6 +151,14 @@ __global__ void __launch_bounds__(256) layout_kernel(LayoutParams p) {
   }
 }
 
+// NaN for every output where a block of the call gave up
+__global__ void __launch_bounds__(512) lost_kernel(OrthoParams o, const unsigned* barrier) {
+  if (*barrier < kGaveUp) return;
+  const int64_t size = o.batch * o.n * o.m;
+  for (int64_t e = (int64_t)blockIdx.x * 512 + threadIdx.x; e < size; e += (int64_t)gridDim.x * 512)
+    ortho_store(o, e, __int_as_float(0x7fffffff));
+}
+
 template <class T, bool UPDATE, int V>
 int start_input(const OrthoGrid& p, cudaStream_t st) {
   const OrthoParams& o = p.o;
@@ -245,7 +257,9 @@ int launch_ortho(const OrthoParams& o, void* workspace, cudaStream_t st) {
         return p.four ? start_input<T, kUpdate, 4>(p, st) : start_input<T, kUpdate, 1>(p, st);
       }))
     return rc;
-  return launch_ortho_split(p, ortho_split_for(p, sms), st);
+  if (int rc = launch_ortho_split(p, ortho_split_for(p, sms), st)) return rc;
+  lost_kernel<<<(unsigned)sms, 512, 0, st>>>(o, p.barrier);
+  return (int)cudaGetLastError();
 }
 
 }  // namespace blitz

@@ -7,6 +7,7 @@
 namespace blitz {
 
 constexpr int kBK = 64;                    // k of one copied box
+constexpr unsigned kGaveUp = 1u << 20;     // above all arrivals: 192 phases of a grid of a few hundred blocks
 constexpr int kBox = 64 * kBK * 2;         // bytes of 64 of its rows of 128 bytes
 
 struct OrthoInfo {  // one matrix's scaling, written while X_0 is laid out
@@ -19,7 +20,7 @@ struct OrthoGrid {
   __half *x[2], *a, *b;   // [2 * batch][n][ld]: high and low terms of each matrix
   double* parts;          // [batch][n_parts] sums of squares
   OrthoInfo* info;        // [batch]
-  unsigned* barrier;      // [0]: arrivals, [1]: gave up
+  unsigned* barrier;      // arrivals, and kGaveUp for a block that gave up
   int n_parts;
   int ldm, ldn;
   int two_in;             // u needs two terms
@@ -47,23 +48,29 @@ __device__ __forceinline__ OrthoTerms ortho_terms(const OrthoGrid& p, int ph) {
   return t;
 }
 
-// every block of the grid has arrived, and what each wrote (for its reads and its copies) is seen
+// every block of the grid has arrived, and what each wrote (for its reads and its copies) is seen.
+// A block that has given up arrives with its word for that in the same addition: whoever passes has
+// seen it, and no block goes on from what it left unfinished.
 __device__ __forceinline__ bool ortho_barrier(unsigned* counter, unsigned target, volatile int* dead, long long limit) {
   fence_async_global();
   __syncthreads();
   if (threadIdx.x == 0) {
-    asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(counter) : "memory");
+    asm volatile("red.release.gpu.global.add.u32 [%0], %1;" ::"l"(counter), "r"(*dead ? kGaveUp + 1 : 1u) : "memory");
     const long long t0 = clock64();
     for (;;) {
       unsigned seen;
       asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(counter) : "memory");
-      if (seen >= target) break;
-      if (*dead || clock64() - t0 > limit || ((volatile unsigned*)counter)[1]) {
+      if (seen >= kGaveUp) {
         *dead = 1;
         break;
       }
+      if (seen >= target) break;
+      if (clock64() - t0 > limit) {
+        *dead = 1;
+        atomicAdd(counter, kGaveUp);
+        break;
+      }
     }
-    if (*dead) atomicExch(counter + 1, 1u);
   }
   __syncthreads();
   fence_async_global();

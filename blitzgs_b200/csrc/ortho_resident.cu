@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) resident_kernel(OrthoP
           tmem_load32(tmem_rows + c, v);
           if (which == 2 && last) {
             // the direction in 32 bits over X, in the order of the matrix's own memory
-            const float f = *dead ? __int_as_float(0x7fffffff) : fx / kScaleB;
+            const float f = fx / kScaleB;
             if (row < n) {
               if (wide) {
                 float* dst = (float*)X + row * stage_stride(m) + c;
@@ -286,9 +286,14 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) resident_kernel(OrthoP
     }
     {
       const int stride = wide ? stage_stride(m) : n;
+      // after the step's last barrier every thread sees the same
+      const bool lost = *dead != 0;
       Walk at(tid * V, THREADS * V, inner);
       ortho_for_out<T, UPDATE, V, 16 / V>(p, base, tid * V, THREADS * V, total, [&](int, float(&d)[V]) {
         load_values<V>((const float*)X + at.o * stride + at.k, d);
+        if (lost)
+#pragma unroll
+          for (int v = 0; v < V; ++v) d[v] = __int_as_float(0x7fffffff);
         at.next();
       });
     }

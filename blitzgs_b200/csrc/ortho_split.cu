@@ -485,9 +485,8 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
     // copies and products of this block that are still in flight end within this time
     const long long t0 = clock64();
     while (clock64() - t0 < 2000000ll) __nanosleep(1000);
-    const int64_t size = p.o.batch * p.o.n * p.o.m;
-    for (int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x; e < size; e += (int64_t)gridDim.x * kThreads)
-      ortho_store(p.o, e, __int_as_float(0x7fffffff));
+    // where it was in the last phase nobody has heard of it: lost_kernel does
+    if (threadIdx.x == 0) atomicAdd(p.barrier, kGaveUp);
   }
   __syncthreads();
   if (warp == 0) tmem_free(tmem_base, kColumns);
