@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(256) read_vector_kernel(QuantParams p) {
   }
 }
 
-// 320k of 8M rows of 45: 109 us for 411 MB (scattered rows open whole sectors), against 36 us for
+// 320k of 8M rows of 45: 113 us for 411 MB (scattered rows open whole sectors), against 36 us for
 // the 238 MB that the rows hold; issue slots 60% busy.  4 or 16 lanes a row took 137 and 131.
 // One group of one row's step.  The moment updates are single rounded operations in
 // the order of the formula (no contraction), so the codes do not depend on how the
@@ -189,10 +189,9 @@ __device__ __forceinline__ void adam8_unit(const Adam8Params& p, int64_t j, int6
     const float g1 = __fmul_rn(w[k], p.grad_scale), root = __fmul_rn(held.y, rs);
     m[k] = __fadd_rn(__fmul_rn(__fmul_rn(held.x, ms), p.b1), __fmul_rn(g1, p.b1c));
     r[k] = __fsqrt_rn(__fadd_rn(__fmul_rn(__fmul_rn(root, root), p.b2), __fmul_rn(__fmul_rn(g1, g1), p.b2c)));
-    // the quotient to 2 units in its last place: it moves the parameter, whose own rounding
-    // is larger, and the moments' codes do not depend on it
+    // each operation rounded once, as in adam.cu
     if (k * LANES < left)
-      param[k * LANES] = __fsub_rn(old[k], __fdividef(__fmul_rn(m[k], p.lr), __fadd_rn(r[k], p.eps)));
+      param[k * LANES] = __fsub_rn(old[k], __fdiv_rn(__fmul_rn(m[k], p.lr), __fadd_rn(r[k], p.eps)));
   }
   const float sm = scale_of<kE4m3, LANES, PER>(m), sr = scale_of<kE4m3, LANES, PER>(r);
   if (row < 0) return;

@@ -42,3 +42,38 @@ def test_both_readers_of_a_nan_code_agree(cuda_device):
                      torch.ones(N, dtype=torch.bool, device=cuda_device), 0.1, 0.9, 0.999, 1e-15, N, M, group=M, seed=1)
     assert held.isnan().nonzero().tolist() == [[1, 7], [2, 44]]
     assert torch.equal(p.isnan(), held.isnan()) and scales.flatten().isnan().tolist() == [False, True, True, False]
+
+
+def _rows(gen, n, M, spread):
+    return torch.randn(n, M, generator=gen) * torch.exp(spread * torch.randn(n, 1, generator=gen))
+
+
+@pytest.mark.parametrize("N,M,group", [(4000, 45, 128), (1000, 12, 12), (500, 100, 50), (200, 300, 256)])
+@pytest.mark.parametrize("form", ["rows", "dense"])
+def test_adam8_parameters_are_the_definitions_bit_for_bit(cuda_device, N, M, group, form):
+    """Every operation of the step is rounded once, the quotient too: the parameter equals the
+    restatement's in single float32 operations, as the 32-bit step's does."""
+    gen = torch.Generator().manual_seed(M)
+    param = torch.randn(N, M, generator=gen)
+    p = param.to(cuda_device)
+    stores = []
+    for x in (_rows(gen, N, M, 1.0) * 1e-3, _rows(gen, N, M, 1.0).abs() * 1e-3):
+        codes = torch.zeros((N, M), dtype=torch.uint8, device=cuda_device).view(torch.float8_e4m3fn)
+        scales = torch.zeros((N, -(-M // group)), device=cuda_device)
+        ops.quant_rows_write(x.to(cuda_device), codes, scales, group=group)
+        stores += [codes, scales]
+    m, r = (ops.quant_rows_read(*stores[k:k + 2], group=group).cpu().numpy() for k in (0, 2))
+    grad = _rows(gen, N, M, 2.0) * 1e-3
+    rows = torch.randperm(N, generator=gen)[:N // 2].sort().values
+    if form == "rows":
+        ops.adam8_update_rows(p, grad[rows].to(cuda_device), *stores, rows.to(cuda_device), 0.01, 0.9, 0.999, 1e-15, N, M,
+                              group=group, seed=3)
+    else:
+        visible = torch.zeros(N, dtype=torch.bool)
+        visible[rows] = True
+        ops.adam8_update(p, grad.to(cuda_device), *stores, visible.to(cuda_device), 0.01, 0.9, 0.999, 1e-15, N, M,
+                         group=group, seed=3)
+    i = rows.numpy()
+    want = param.numpy().copy()
+    want[i] = O.adam8(want, grad.numpy()[i], m[i], r[i], i, 0.01, 0.9, 0.999, 1e-15, 3, group)[0]
+    assert np.array_equal(p.cpu().numpy(), want)
