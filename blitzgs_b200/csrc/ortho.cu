@@ -15,7 +15,7 @@
 // bf16 terms would need three for that.  16-bit inputs are exact in one term, so step 0
 // reads one of X; every other operand has two, whatever type the result is rounded to.
 // Everything is scaled by powers of two into
-// f16's range: |X_ij| <= 1.9 by 2^14, |A_ij| <= 3.7 by 2^14, |B_ij| < 7.9 by 2^13
+// f16's range: |X_ij| <= 1.9 by 2^14 (by more where X is tiny throughout, see OrthoInfo), |A_ij| <= 3.7 by 2^14, |B_ij| < 7.9 by 2^13
 // (the caller's coefficients are checked to keep to that).
 //
 // Which kernel runs goes by size: registers or one block's shared memory (ortho_small.cu), one
@@ -80,7 +80,7 @@ struct LayoutParams {
 template <class T, bool UPDATE, int V>
 __global__ void __launch_bounds__(256) layout_kernel(LayoutParams p) {
   __shared__ float tile[64 * 65];
-  __shared__ float up_shared;
+  __shared__ float2 up_shared;
   const OrthoParams& o = p.o;
   const int n = (int)o.n, m = (int)o.m, tid = threadIdx.x;
   const int tj = p.ldm / 64, per = (n + 63) / 64 * tj;
@@ -120,8 +120,7 @@ __global__ void __launch_bounds__(256) layout_kernel(LayoutParams p) {
 #pragma unroll
     for (int k = 16; k > 0; k >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, k);
     if (tid == 0) {
-      OrthoInfo info;
-      ortho_scaling(sqrt(sq), o.eps, info.up, info.alpha);
+      const OrthoInfo info = ortho_scaling(sqrt(sq), o);
       up_shared = info.up;
       if (r == 0) p.info[b] = info;
     }
@@ -133,7 +132,7 @@ __global__ void __launch_bounds__(256) layout_kernel(LayoutParams p) {
       for (int e = 0; e < 4; ++e) tile[(q + e) * 65 + (tid >> 4) + 16 * k] = u[k][e];
   }
   __syncthreads();
-  const float up = up_shared;
+  const float2 up = up_shared;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int x = (tid >> 4) + 16 * k;
@@ -143,8 +142,8 @@ __global__ void __launch_bounds__(256) layout_kernel(LayoutParams p) {
       for (int e = 0; e < 4; ++e) u[k][e] = tile[x * 65 + q + e];
     }
     uint2 hi, lo;
-    hi.x = split2(u[k][0] * up, u[k][1] * up, lo.x);
-    hi.y = split2(u[k][2] * up, u[k][3] * up, lo.y);
+    hi.x = split2(u[k][0] * up.x * up.y, u[k][1] * up.x * up.y, lo.x);
+    hi.y = split2(u[k][2] * up.x * up.y, u[k][3] * up.x * up.y, lo.y);
     __half* dst = p.x + ((2 * b) * n + i0 + x) * (int64_t)p.ldm + j0 + q;
     *(uint2*)dst = hi;
     if (p.two_in) *(uint2*)(dst + (int64_t)n * p.ldm) = lo;

@@ -8,21 +8,49 @@
 
 namespace blitz {
 
-// the powers of two that X, A and B are scaled by in f16 terms (see ortho.cu)
+// the powers of two that X (at least, see OrthoInfo), A and B are scaled by in f16 terms (see ortho.cu)
 constexpr float kScaleX = 16384.0f, kScaleA = 16384.0f, kScaleB = 8192.0f;
 
-// how u with 2-norm `norm` is scaled into f16: it is stored as u * up, exactly,
-// with norm * up in [2^13, 2^14), and X_0 is alpha times that
-__device__ __forceinline__ void ortho_scaling(double norm, float eps, float& up, float& alpha) {
-  int e = norm > 0.0 && norm <= 1e300 ? 14 - (ilogb(norm) + 1) : 0;
-  e = max(-126, min(120, e));
-  up = ldexpf(1.0f, e);
+// How one matrix is scaled into f16.  u with 2-norm `norm` is stored as u * up.x * up.y, exactly
+// (two factors, since 2^163 is no float), with norm times that in [2^13, 2^14).  X_1 and what
+// follows are stored times x = 2^14 2^k, with k > 0 where u is so much smaller than eps that the
+// iterates stay small: they would lie among f16's denormals (in 40 x 60 with eps = 1e-7, 1.6e-3 off
+// for a norm of 1e-15).  X_0 times x is `first` times what is stored of u; inv is 1 / x.
+struct OrthoInfo {
+  float2 up;
+  float first, inv;
+};
+__device__ __forceinline__ OrthoInfo ortho_scaling(double norm, const OrthoParams& p) {
+  OrthoInfo info;
+  const int e = max(-126, norm > 0.0 && norm <= 1e300 ? 14 - (ilogb(norm) + 1) : 0);
+  info.up = make_float2(ldexpf(1.0f, min(e, 80)), ldexpf(1.0f, max(e - 80, 0)));
+  int k = 0;
+  if (norm < (double)p.eps) {
+    // bounds of the iterates: a step multiplies singular values up to s by at most
+    // |a| + |b| s^2 + |c| s^4, and they stay below 1.85 (checked by the caller)
+    double s = norm / (norm + (double)p.eps), most = s;
+    for (int i = 0; i < p.steps; ++i) {
+      const double l = s * s;
+      s = fmin(s * (fabs((double)p.a) + l * (fabs((double)p.b) + l * fabs((double)p.c))), 1.85);
+      most = fmax(most, s);
+    }
+    if (most > 0.0) k = max(0, min(100, ilogb(1.85 / most)));
+  }
+  info.inv = ldexpf(1.0f / kScaleX, -k);
   // zeros stay zeros, whatever eps is
-  alpha = norm == 0.0 ? 0.0f : (float)(1.0 / ((norm + (double)eps) * ldexp(1.0, e)));
+  info.first = norm == 0.0 ? 0.0f : (float)(1.0 / ((norm + (double)p.eps) * ldexp((double)info.inv, e)));
+  return info;
 }
 
 // whether u needs two f16 terms
 __host__ __device__ inline bool ortho_two_in(const OrthoParams& p) { return p.param || p.g_type == kValueF32; }
+
+// What the kernels that stay in 32 bits multiply u with 2-norm `norm` by, in two factors: alone
+// 1 / norm would be infinite for norms below 2^-128.  .y is 1 but for the smallest.
+__device__ __forceinline__ float2 ortho_inverse(double norm, float eps) {
+  const double s = norm == 0.0 ? 0.0 : 1.0 / (norm + (double)eps);
+  return s > 0x1p100 ? make_float2((float)(s * 0x1p-80), 0x1p80f) : make_float2((float)s, 1.0f);
+}
 
 // 32 bytes of global memory, a whole sector, by one lane
 __device__ __forceinline__ void store32(void* p, const uint32_t (&v)[8]) {

@@ -10,16 +10,12 @@ constexpr int kBK = 64;                    // k of one copied box
 constexpr unsigned kGaveUp = 1u << 20;     // above all arrivals: 192 phases of a grid of a few hundred blocks
 constexpr int kBox = 64 * kBK * 2;         // bytes of 64 of its rows of 128 bytes
 
-struct OrthoInfo {  // one matrix's scaling, written while X_0 is laid out
-  float up, alpha;  // X_0 is stored as u * up; alpha = 1 / ((|u|_F + eps) * up)
-};
-
 struct OrthoGrid {
   OrthoParams o;
   CUtensorMap map_x[2], map_a, map_b;  // boxes of 64 rows (128 rows a box took a quarter longer)
   __half *x[2], *a, *b;   // [2 * batch][n][ld]: high and low terms of each matrix
   double* parts;          // [batch][n_parts] sums of squares
-  OrthoInfo* info;        // [batch]
+  OrthoInfo* info;        // [batch], written while X_0 is laid out
   unsigned* barrier;      // arrivals, and kGaveUp for a block that gave up
   int n_parts;
   int ldm, ldn;

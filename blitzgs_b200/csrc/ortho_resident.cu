@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) resident_kernel(OrthoP
   __shared__ uint32_t tmem_base;
   __shared__ int dead_flag;
   __shared__ double sums[THREADS / 32];
-  __shared__ float2 scaling;
+  __shared__ OrthoInfo scaling;
   volatile int* dead = &dead_flag;
   uint8_t* X = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
   const int n = (int)p.n, m = (int)p.m, tid = threadIdx.x, lane = tid & 31;
@@ -170,12 +170,10 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) resident_kernel(OrthoP
       __syncthreads();
       if (tid == 0) {
         for (int w = 1; w < THREADS / 32; ++w) sq += sums[w];
-        float up, alpha;
-        ortho_scaling(sqrt(sq), p.eps, up, alpha);
-        scaling = make_float2(up, alpha);
+        scaling = ortho_scaling(sqrt(sq), p);
       }
       __syncthreads();
-      const float up = scaling.x;
+      const float2 up = scaling.up;
       // whole rows of 128 bytes, so the swizzle does not matter
       for (int e = tid; e < l.x_term / 16; e += THREADS) {
         uint4* hi = (uint4*)X + e;
@@ -185,8 +183,8 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) resident_kernel(OrthoP
         float x[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          x[2 * k] = __uint_as_float(__byte_perm(ls[k], hs[k], 0x5410)) * up;
-          x[2 * k + 1] = __uint_as_float(__byte_perm(ls[k], hs[k], 0x7632)) * up;
+          x[2 * k] = __uint_as_float(__byte_perm(ls[k], hs[k], 0x5410)) * up.x * up.y;
+          x[2 * k + 1] = __uint_as_float(__byte_perm(ls[k], hs[k], 0x7632)) * up.x * up.y;
         }
         uint4 nh, nl;
         split8(x, nh, nl);
@@ -196,13 +194,13 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) resident_kernel(OrthoP
     }
     fence_async_shared();
     __syncthreads();
-    const float alpha = scaling.y;
+    const float first = scaling.first, inv = scaling.inv;
 
 #pragma unroll 1
     for (int s = 0; s < p.steps; ++s) {
       const bool two_x = s > 0 || two_in;
       const bool last = s + 1 == p.steps;
-      const float fx = s == 0 ? alpha : 1.0f / kScaleX;
+      const float from = s == 0 ? first : 1.0f, fx = from * inv;
 #pragma unroll 1
       for (int which = 0; which < 3; ++which) {
         if (warp == 0) {
@@ -249,7 +247,7 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) resident_kernel(OrthoP
           uint8_t* dst = which == 2 ? X : A;
           const int term = which == 2 ? l.x_term : l.a_term;
           const float f = which == 0 ? fx * fx * kScaleA : which == 1 ? p.c * (kScaleB / (kScaleA * kScaleA))
-                                                                     : fx * (kScaleX / kScaleB);
+                                                                     : from / kScaleB;
           const float fb = p.b * (kScaleB / kScaleA);
 #pragma unroll
           for (int k = 0; k < 32; k += 8) {

@@ -68,11 +68,11 @@ __global__ void __launch_bounds__(128) thin_kernel(OrthoParams p, int gap) {
   }
 #pragma unroll
   for (int o = LANES / 2; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
-  const float scale = sq == 0.0 ? 0.0f : (float)(1.0 / (sqrt(sq) + (double)p.eps));
+  const float2 scale = ortho_inverse(sqrt(sq), p.eps);
 #pragma unroll
   for (int k = 0; k < COLS; ++k)
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i][k] *= scale;
+    for (int i = 0; i < N; ++i) x[i][k] *= scale.y, x[i][k] *= scale.x;
   for (int s = 0; s < p.steps; ++s) {
     float A[N][N], B[N][N];
 #pragma unroll
@@ -263,8 +263,8 @@ __global__ void __launch_bounds__(THREADS) block_kernel(OrthoParams p) {
     block_sync<THREADS>();
     sq = 0.0;
     for (int w = 0; w < THREADS / 32; ++w) sq += sums[w];
-    const float scale = sq == 0.0 ? 0.0f : (float)(1.0 / (sqrt(sq) + (double)p.eps));
-    for (int e = tid; e < l.np * l.ldx; e += THREADS) X[e] *= scale;
+    const float2 scale = ortho_inverse(sqrt(sq), p.eps);
+    for (int e = tid; e < l.np * l.ldx; e += THREADS) X[e] = X[e] * scale.y * scale.x;
     block_sync<THREADS>();
     for (int s = 0; s < p.steps; ++s) {
       const auto gram = [](float x, int, int) { return x; };

@@ -53,3 +53,24 @@ def matrices(shape, dtype, device, seed=0):
 def test_directions_of_16_bits_are_exact_but_for_their_rounding(cuda_device, shape, dtype):
     g = matrices(shape, dtype, cuda_device)
     assert beyond_rounding(ops.orthogonalize(g), formula(g)) <= 1e-5
+
+
+@pytest.mark.parametrize("shape", [(1, 3), (12, 3), (9, 14), (24, 40), (100, 250), (200, 150), (150, 160)])
+def test_updates_far_smaller_than_eps(cuda_device, shape):
+    """The direction is then small throughout (a^5 |u| / eps), and as exact."""
+    base = matrices(shape, torch.float32, "cpu")
+    for norm in (1e-9, 1e-10, 1e-12, 1e-14, 1e-17, 1e-25, 1e-33):
+        g = (base * (norm / base.norm())).to(cuda_device)
+        for steps in (1, 2, 5):
+            got = ops.orthogonalize(g, steps=steps)
+            assert beyond_rounding(got, formula(g, steps=steps)) <= 1e-5, (norm, steps)
+
+
+@pytest.mark.parametrize("shape", [(1, 3), (12, 3), (9, 14), (24, 40), (100, 250), (200, 150), (150, 160)])
+def test_the_smallest_and_largest_updates_without_eps(cuda_device, shape):
+    """The direction of what 32 bits hold, down to numbers that are denormal themselves."""
+    base = matrices(shape, torch.float32, "cpu").double()
+    for norm in (1e-20, 1e-30, 1e-34, 1e-37, 3e-39, 1e-41, 1e30, 1e38):
+        g = (base * (norm / base.norm())).float().to(cuda_device)
+        got = ops.orthogonalize(g, eps=0.0)
+        assert beyond_rounding(got, formula(g, eps=0.0)) <= 1e-5, norm
