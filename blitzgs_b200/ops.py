@@ -1001,7 +1001,7 @@ def quant_rows_write(values, codes, scales, rows=None, *, group, seed=None):
     (int8, or float8_e4m3fn with power-of-two scales) and float32 scales
     [N, ceil(D / group)] (blitz_quant_rows_write).  Rows outside [0, N) are
     skipped.  ``seed`` (an int or an int64 tensor of one element) dithers the
-    rounding; None rounds to nearest even."""
+    rounding; None rounds to nearest even.  What is stored has no graph."""
     _same_device(values, codes, scales, rows)
     N, D, kind = _code_rows(codes, scales, group, "quant_rows_write")
     n = N if rows is None else rows.numel()
@@ -1021,9 +1021,17 @@ def quant_rows_write(values, codes, scales, rows=None, *, group, seed=None):
     TIMER.end(tok, n_rows=n, D=D)
 
 
+def _no_graph(t, what):
+    """What returns a new tensor and has no backward refuses to cut a graph unsaid."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{what} has no backward: call it under torch.no_grad(), or with detached tensors")
+
+
 def quant_rows_read(codes, scales, rows=None, *, group, dtype=torch.float32):
     """The rows (int64 [n]; None: all) of an 8-bit store as values [n, D] in
-    dtype (blitz_quant_rows_read); rows outside [0, N) read as zeros."""
+    dtype (blitz_quant_rows_read); rows outside [0, N) read as zeros.  Not
+    differentiable: scales that require a gradient are refused."""
+    _no_graph(scales, "quant_rows_read")
     _same_device(codes, scales, rows)
     N, D, kind = _code_rows(codes, scales, group, "quant_rows_read")
     if dtype not in _VALUE_TYPES:
@@ -1106,7 +1114,9 @@ def orthogonalize(g, *, steps=5, coefficients=ORTHO_COEFFICIENTS, eps=1e-7):
     """The direction of each matrix of g [..., rows, cols] (float32, bfloat16
     or float16): its singular values driven towards 1 by ``steps`` Newton-Schulz
     steps (blitz_orthogonalize).  Returns a new tensor of g's type, within
-    about 1e-5 (2-norm) of the formula before its rounding to that type."""
+    about 1e-5 (2-norm) of the formula before its rounding to that type.  Not
+    differentiable: where gradients are on, a g that requires one is refused."""
+    _no_graph(g, "orthogonalize")
     _same_device(g)
     if g.dtype not in _VALUE_TYPES:
         raise RuntimeError(f"orthogonalize: values are of 32 or 16 bits, got {g.dtype}")
