@@ -958,6 +958,13 @@ def _same_device(first, *others):
         raise RuntimeError(f"tensors on {first.device}, but the current device is cuda:{torch.cuda.current_device()}")
 
 
+def _written(*tensors):
+    """Raise the version counters of tensors that a kernel has written, as torch's own in-place
+    operations do: autograd then refuses a backward pass that needs what they held, and
+    caches keyed by the version see the change."""
+    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+
+
 def _code_rows(codes, scales, group, what):
     """(N, D, kind) of a store's contiguous codes [N, D] (int8 or
     float8_e4m3fn) and scales [N, ceil(D / group)]."""
@@ -1019,6 +1026,7 @@ def quant_rows_write(values, codes, scales, rows=None, *, group, seed=None):
               ptr(codes), ptr(scales), kind, ptr(rows), n, N, D, int(group),
               int(seed is not None), s, ptr(s_ptr), _lib.stream_ptr())
     TIMER.end(tok, n_rows=n, D=D)
+    _written(codes, scales)
 
 
 def _no_graph(t, what):
@@ -1067,6 +1075,7 @@ def _adam8(param, grad, m_codes, m_scales, r_codes, r_scales, visible, rows, n, 
               ptr(visible), ptr(rows), n, float(grad_scale), float(lr), float(b1), 1.0 - float(b1), float(b2),
               1.0 - float(b2), float(eps), N, M, int(group), s, ptr(s_ptr), _lib.stream_ptr())
     TIMER.end(tok, N=N, M=M, n_rows=n)
+    _written(param, m_codes, m_scales, r_codes, r_scales)
 
 
 def adam8_update(param, grad, m_codes, m_scales, r_codes, r_scales, visible, lr, b1, b2, eps, N, M, *, group, seed,
@@ -1163,3 +1172,4 @@ def orthogonal_update(param, grad, momentum, lr, *, beta=0.95, nesterov=True, we
               cols, int(steps), a, b, c, float(eps), float(beta), 1.0 - float(beta), int(bool(nesterov)),
               1.0 - float(lr) * float(weight_decay), float(lr) * float(scale), ptr(ws), need, _lib.stream_ptr())
     TIMER.end(tok, batch=batch, rows=rows, cols=cols)
+    _written(param, momentum)

@@ -34,3 +34,45 @@ def test_what_has_no_backward_refuses_tensors_that_want_one():
             call()
     with pytest.raises(RuntimeError, match="CUDA"):
         ops.orthogonalize(g.detach())
+
+
+@pytest.fixture
+def no_kernels(monkeypatch):
+    """The wrappers on CPU tensors, up to the calls of the library, which do nothing."""
+    monkeypatch.setattr(ops, "_same_device", lambda *t: None)
+    monkeypatch.setattr(ops, "ptr", lambda t: None)
+    monkeypatch.setattr(_lib, "call", lambda *a: 0)
+    monkeypatch.setattr(_lib, "stream_ptr", lambda: None)
+
+
+def test_in_place_operators_raise_the_versions_of_what_they_write(no_kernels):
+    """So that a backward pass through a parameter that has been stepped since is refused, as after
+    torch's own optimizers, and no cache keyed by the version answers with what was there before."""
+    N, M = 6, 45
+
+    def store():
+        return torch.zeros(N, M, dtype=torch.uint8).view(torch.float8_e4m3fn), torch.zeros(N, 1)
+
+    p, m, r, rows = torch.nn.Parameter(torch.ones(N, M)), store(), store(), torch.arange(N)
+    args = (0.1, 0.9, 0.999, 1e-15, N, M)
+    steps = {"adam8": lambda: ops.adam8_update(p, torch.ones(N, M), *m, *r, torch.ones(N).bool(), *args, group=M, seed=0),
+             "rows": lambda: ops.adam8_update_rows(p, torch.ones(N, M), *m, *r, rows, *args, group=M, seed=0)}
+    for step in steps.values():
+        loss = (p * p).sum()
+        before = [t._version for t in (p, *m, *r)]
+        step()
+        assert all(t._version > v for t, v in zip((p, *m, *r), before))
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    w, M0 = torch.nn.Parameter(torch.ones(5, 6)), torch.zeros(5, 6)
+    loss, before = (w * w).sum(), (w._version, M0._version)
+    ops.orthogonal_update(w, torch.ones(5, 6), M0, 0.1)
+    assert w._version > before[0] and M0._version > before[1]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    before = [t._version for t in m]
+    ops.quant_rows_write(torch.ones(N, M), *m, group=M)
+    assert all(t._version > v for t, v in zip(m, before))
+    with torch.inference_mode():
+        c, s = store()
+        ops.quant_rows_write(torch.ones(N, M), c, s, group=M)
