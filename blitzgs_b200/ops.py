@@ -961,8 +961,9 @@ def _same_device(first, *others):
 def _written(*tensors):
     """Raise the version counters of tensors that a kernel has written, as torch's own in-place
     operations do: autograd then refuses a backward pass that needs what they held, and
-    caches keyed by the version see the change."""
-    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+    caches keyed by the version see the change.  (Tensors made in inference mode have none, and
+    are passed over.)"""
+    torch._C._increment_version(tensors)  # torch.autograd.graph.increment_version, without its checks
 
 
 def _code_rows(codes, scales, group, what):
