@@ -81,6 +81,14 @@ def _codes_back(state, keys):
                 st[k] = st[k].to(torch.uint8)
 
 
+def _not_captured(param, what):
+    """A captured step would be replayed with one seed: rounded up or down at the same places every
+    time, a moving average drifts from its values or stands still."""
+    if param.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{what} takes its seed from the host's step count and cannot be captured into a graph: "
+                           "capture the operators of ops with a seed tensor that the graph counts up")
+
+
 class SparseGaussianAdam8bit(SparseGaussianAdam):
     """``SparseGaussianAdam`` with both moments in 8 bits: the same constructor,
     ``step(visibility, N, bsz)``, learning-rate correction, sparse gradients and
@@ -106,6 +114,7 @@ class SparseGaussianAdam8bit(SparseGaussianAdam):
         M = param.numel() // n
         if M < 8:
             return super()._update(param, state, n, visibility, lr, eps, scale)
+        _not_captured(param, "SparseGaussianAdam8bit")
         group = self.values_per_scale
         if len(state) == 0:
             state["step"] = torch.tensor(0.0, dtype=torch.float32)
@@ -168,6 +177,7 @@ class OrthogonalMomentum(torch.optim.Optimizer):
                 state["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
             ops.orthogonal_update(p, p.grad, state["momentum_buffer"], group["lr"], **how)
             return
+        _not_captured(p, "OrthogonalMomentum with momentum_bits=8")
         rows, cols, values = p.numel() // p.shape[-1], p.shape[-1], min(p.shape[-1], 128)
         if len(state) == 0:
             state["step"] = torch.tensor(0.0, dtype=torch.float32)

@@ -1,0 +1,52 @@
+"""The optimizers of blitzgs_b200.optim in uses that could go wrong unnoticed."""
+import pytest
+import torch
+
+from blitzgs_b200 import optim
+
+pytestmark = pytest.mark.gpu
+
+
+def _captures(step):
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        step()
+    return graph
+
+
+def test_steps_that_round_by_the_hosts_count_are_not_captured(cuda_device):
+    """A replayed seed would round alike every time.  What is refused leaves no trace, and the
+    next step outside of a capture is the first."""
+    p, q = torch.nn.Parameter(torch.zeros(50, 45, device=cuda_device)), torch.nn.Parameter(
+        torch.ones(20, 30, device=cuda_device))
+    p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    visible = torch.ones(50, dtype=torch.bool, device=cuda_device)
+    adam = optim.SparseGaussianAdam8bit([{"params": [p], "lr": 0.1}], 0.0, 1e-15)
+    mat = optim.OrthogonalMomentum([q], momentum_bits=8)
+    for step in (lambda: adam.step(visibility=visible, N=50), mat.step):
+        with pytest.raises(RuntimeError, match="captured"):
+            _captures(step)
+        torch.cuda.synchronize()
+    assert len(adam.state[p]) == 0 and len(mat.state[q]) == 0 and (p == 0).all() and (q == 1).all()
+    adam.step(visibility=visible, N=50)
+    mat.step()
+    assert int(adam.state[p]["step"]) == 1 and (p < 0).all() and not (q == 1).all()
+
+
+def test_a_captured_step_of_matrices_with_32_bit_momentum_repeats_the_eager_one(cuda_device):
+    gen = torch.Generator().manual_seed(0)
+    start, grad = torch.randn(3, 40, 60, generator=gen), torch.randn(3, 40, 60, generator=gen)
+    params, opts = [], []
+    for _ in range(2):
+        params.append(torch.nn.Parameter(start.to(cuda_device)))
+        params[-1].grad = grad.to(cuda_device)
+        opts.append(optim.OrthogonalMomentum([params[-1]], lr=0.05))
+        opts[-1].step()  # makes the state
+    graph = _captures(opts[1].step)
+    for _ in range(3):
+        opts[0].step()
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(params[0], params[1]) and torch.equal(*(o.state[p]["momentum_buffer"]
+                                                               for o, p in zip(opts, params)))
