@@ -109,13 +109,17 @@ class SparseGaussianAdam8bit(SparseGaussianAdam):
         if not 1 <= group <= 256:
             raise ValueError(f"a group holds 1 to 256 values, got {group}")
         self.values_per_scale = group
+        # saved and loaded with the state that is laid out by it
+        for g in self.param_groups:
+            g["values_per_scale"] = group
 
     def _update(self, param, state, n, visibility, lr, eps, scale):
         M = param.numel() // n
         if M < 8:
             return super()._update(param, state, n, visibility, lr, eps, scale)
         _not_captured(param, "SparseGaussianAdam8bit")
-        group = self.values_per_scale
+        group = next((g.get("values_per_scale", self.values_per_scale) for g in self.param_groups
+                      if g["params"][0] is param), self.values_per_scale)
         if len(state) == 0:
             state["step"] = torch.tensor(0.0, dtype=torch.float32)
             for k in ("exp_avg", "exp_root"):

@@ -1,9 +1,12 @@
 """CPU checks of the 8-bit optimizer state and the orthogonalised updates where they could go
 wrong unnoticed: sizes past 32 bits and the wrappers' and optimizers' refusals."""
+import copy
+
 import pytest
 import torch
 
-from blitzgs_b200 import _lib, ops
+from blitzgs_b200 import _lib, ops, optim
+from tests.test_cpu_optim import fake_kernels  # noqa: F401 (a fixture)
 
 EINVAL = 10001
 
@@ -76,3 +79,42 @@ def test_in_place_operators_raise_the_versions_of_what_they_write(no_kernels):
     with torch.inference_mode():
         c, s = store()
         ops.quant_rows_write(torch.ones(N, M), c, s, group=M)
+
+
+def _stepped(opt, p, grads):
+    for g in grads:
+        p.grad = g.clone()
+        opt.step(visibility=torch.ones(p.shape[0]).bool(), N=p.shape[0])
+    return p
+
+
+@pytest.mark.parametrize("other", [64, 70, 128])
+def test_a_loaded_state_keeps_the_groups_it_was_made_with(fake_kernels, other):  # noqa: F811
+    """100 values in groups of 50 and of 64 have two scales each, but not of the same values: an
+    optimizer made with other groups goes on with the loaded ones."""
+    gen = torch.Generator().manual_seed(0)
+    start, grads = torch.randn(6, 100, generator=gen), torch.randn(4, 6, 100, generator=gen)
+    p, q = torch.nn.Parameter(start.clone()), torch.nn.Parameter(start.clone())
+    first = optim.SparseGaussianAdam8bit([{"params": [p], "lr": 0.01}], 0.0, 1e-15, group=50)
+    _stepped(first, p, grads[:2])
+    with torch.no_grad():
+        q.copy_(p)
+    second = optim.SparseGaussianAdam8bit([{"params": [q], "lr": 0.01}], 0.0, 1e-15, group=other)
+    # as a file would: torch itself loads tensors of the right type without copying them
+    second.load_state_dict(copy.deepcopy(first.state_dict()))
+    assert torch.equal(_stepped(first, p, grads[2:]), _stepped(second, q, grads[2:]))
+    for k, t in first.state[p].items():
+        assert torch.equal(t, second.state[q][k])
+
+
+def test_groups_of_a_state_saved_without_their_size_are_the_optimizers(fake_kernels):  # noqa: F811
+    """State that names no group size, and parameters added later."""
+    p, q = torch.nn.Parameter(torch.zeros(6, 100)), torch.nn.Parameter(torch.zeros(6, 100))
+    opt = optim.SparseGaussianAdam8bit([{"params": [p], "lr": 0.01}], 0.0, 1e-15, group=25)
+    state = opt.state_dict()
+    del state["param_groups"][0]["values_per_scale"]
+    opt.load_state_dict(state)
+    opt.add_param_group({"params": [q], "lr": 0.01})
+    q.grad = torch.ones(6, 100)
+    _stepped(opt, p, torch.ones(1, 6, 100))
+    assert opt.state[p]["exp_avg_scales"].shape == opt.state[q]["exp_avg_scales"].shape == (6, 4)
