@@ -250,13 +250,16 @@ int launch_ortho(const OrthoParams& o, void* workspace, cudaStream_t st) {
     if (int rc = make_map(&p.map_x[i], p.x[i], o.m, o.n, q.ldm, o.batch)) return rc;
   if (int rc = make_map(&p.map_a, p.a, o.n, o.n, q.ldn, o.batch)) return rc;
   if (int rc = make_map(&p.map_b, p.b, o.n, o.n, q.ldn, o.batch)) return rc;
+  // what can fail does so before the first kernel advances the momentum
+  const int split = ortho_split_for(p, sms);
+  if (int rc = ortho_split_ready(split)) return rc;
   if (int rc = ortho_dispatch(o, [&](auto type, auto update) {
         using T = decltype(type);
         constexpr bool kUpdate = decltype(update)::value;
         return p.four ? start_input<T, kUpdate, 4>(p, st) : start_input<T, kUpdate, 1>(p, st);
       }))
     return rc;
-  if (int rc = launch_ortho_split(p, ortho_split_for(p, sms), st)) return rc;
+  if (int rc = launch_ortho_split(p, split, st)) return rc;
   lost_kernel<<<(unsigned)sms, 512, 0, st>>>(o, p.barrier);
   return (int)cudaGetLastError();
 }

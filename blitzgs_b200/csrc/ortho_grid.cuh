@@ -74,7 +74,9 @@ __device__ __forceinline__ bool ortho_barrier(unsigned* counter, unsigned target
 }
 
 int launch_ortho_split(const OrthoGrid& p, int split, cudaStream_t st);
-// the split that launch_ortho_split takes for this size (0: the other kernel), and its clusters
+// an error if a split's kernel cannot be launched here at all
+int ortho_split_ready(int split);
+// the split that launch_ortho_split takes for this size
 int ortho_split_for(const OrthoGrid& p, int sms);
 
 }  // namespace blitz

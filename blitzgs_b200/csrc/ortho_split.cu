@@ -546,10 +546,16 @@ int start(const OrthoGrid& p, int sms, cudaStream_t st) {
   const int64_t tiles = p.o.batch * std::max(mt * nt, mt * (mt + 1) / 2);
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr[2];
-  const int k = (int)std::min<int64_t>(clusters<S>(sms), tiles);
+  int k = (int)std::min<int64_t>(clusters<S>(sms), tiles);
   if (k < 1) return (int)cudaErrorLaunchOutOfResources;
-  if (int rc = configure<S>(cfg, attr, S * k, st)) return rc;
-  return (int)cudaLaunchKernelEx(&cfg, split_kernel<S>, p);
+  // Where the context has fewer SMs than the device (a part of it set aside for others), as
+  // many blocks as it takes: a grid of any size goes through all tiles.
+  for (;; k = (k + 1) / 2) {
+    if (int rc = configure<S>(cfg, attr, S * k, st)) return rc;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, split_kernel<S>, p);
+    if (e != cudaErrorCooperativeLaunchTooLarge || k == 1) return (int)e;
+    cudaGetLastError();
+  }
 }
 
 }  // namespace
@@ -578,6 +584,14 @@ int ortho_split_for(const OrthoGrid& p, int sms) {
     }
   }
   return best;
+}
+
+int ortho_split_ready(int split) {
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr[2];
+  return split == 1   ? configure<1>(cfg, attr, 1, nullptr)
+         : split == 2 ? configure<2>(cfg, attr, 2, nullptr)
+                      : configure<4>(cfg, attr, 4, nullptr);
 }
 
 int launch_ortho_split(const OrthoGrid& p, int split, cudaStream_t st) {

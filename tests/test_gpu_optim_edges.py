@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from blitzgs_b200 import optim
+from blitzgs_b200 import ops, optim
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +50,31 @@ def test_a_captured_step_of_matrices_with_32_bit_momentum_repeats_the_eager_one(
     torch.cuda.synchronize()
     assert torch.equal(params[0], params[1]) and torch.equal(*(o.state[p]["momentum_buffer"]
                                                                for o, p in zip(opts, params)))
+
+
+@pytest.mark.parametrize("shape", [(777, 201), (1024, 1024), (2, 300, 260)])
+def test_an_update_in_a_part_of_the_gpu_equals_one_on_the_whole(cuda_device, shape):
+    """A context with 24 SMs takes fewer blocks of the kernel that needs all of its blocks at once.
+    (The launch used to be refused there, after the momentum had been advanced.)"""
+    from torch.cuda import green_contexts
+    if not green_contexts.SUPPORTED:
+        pytest.skip("torch was built without green contexts")
+    gen = torch.Generator().manual_seed(0)
+    param, grad, momentum = (torch.randn(shape, generator=gen).to(cuda_device) for _ in range(3))
+
+    def update():
+        p, M = param.clone(), momentum.clone()
+        ops.orthogonal_update(p, grad, M, 0.1)
+        torch.cuda.synchronize()
+        return p, M
+
+    want = update()
+    part = green_contexts.GreenContext.create(num_sms=24, device_id=0)
+    part.set_context()
+    try:
+        with torch.cuda.stream(part.Stream()):
+            got = update()
+    finally:
+        part.pop_context()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert all(torch.equal(a, b) for a, b in zip(update(), want))
