@@ -74,3 +74,48 @@ def test_the_smallest_and_largest_updates_without_eps(cuda_device, shape):
         g = (base * (norm / base.norm())).float().to(cuda_device)
         got = ops.orthogonalize(g, eps=0.0)
         assert beyond_rounding(got, formula(g, eps=0.0)) <= 1e-5, norm
+
+
+# Of an error d in each operand of a product (two f16 terms: 2^-23 of X, A and B, and the low * low
+# product left out, 2^-22: together 2^-22 in the mean), what arises in step k reaches the result
+# multiplied by at most a^(5 - k) |X_k| / |X_5|.  For n of some hundred rows these factors are about
+# 21, 21, 21, 20, 6 and 2; independent errors add up in squares, so to 43 * 2^-22 = 1e-5 if every
+# direction is a weak one.  Summed without the registers' rounding, 1024 columns alone leave 4e-5.
+STATED = 1e-5
+
+
+@pytest.mark.parametrize("shape", [
+    (1, 1), (1, 7), (2, 2), (15, 3), (4, 17), (3, 64), (4, 512), (4, 513), (9, 31), (16, 16), (16, 33), (50, 16, 16),
+    (17, 17), (63, 64), (64, 65), (33, 200), (64, 700), (127, 129), (128, 128), (300, 70, 66), (128, 256), (129, 257),
+    (200, 1000), (513, 130), (300, 300), (700, 640), (20, 150, 260), (40, 257, 130), (130, 5000), (1030, 1100),
+    (1400, 1290), (1153, 2177), (2048, 1024), (3000, 3000), (2999, 3101)])
+def test_32_bit_directions(cuda_device, shape):
+    for seed in range(2):
+        g = matrices(shape, torch.float32, cuda_device, seed)
+        want = formula(g)
+        assert float((ops.orthogonalize(g).double() - want).norm() / want.norm()) <= STATED
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (12, 3, 4), (100, 15, 3), (6, 16, 16), (20, 30), (3, 64, 64), (128, 256),
+                                   (256, 128), (150, 200), (260, 200), (150, 201), (201, 150), (20, 150, 260),
+                                   (7, 300, 130), (1400, 1292), (1292, 1400), (1401, 1291), (1291, 1401), (2048, 1024)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("nesterov", [True, False])
+def test_updates(cuda_device, shape, dtype, nesterov):
+    """Wide and tall, rows of whole fours of values and not, one tile to more than the grid has blocks:
+    the momentum bit for bit, the parameter within the direction's stated error times lr scale and its
+    own roundings (the two products' and the sum's, 2^-24 each of at most |param| + |step|)."""
+    g = matrices(shape, dtype, cuda_device)
+    M0, p0 = matrices(shape, torch.float32, cuda_device, 1), matrices(shape, torch.float32, cuda_device, 2) * 100
+    p, M = p0.clone(), M0.clone()
+    lr, beta, decay = 0.02, 0.95, 0.1
+    ops.orthogonal_update(p, g, M, lr, beta=beta, nesterov=nesterov, weight_decay=decay)
+    h = g.float() * (1 - beta)
+    want_M = M0 * beta + h
+    assert torch.equal(M, want_M)
+    o = formula(h + want_M * beta if nesterov else want_M)
+    alpha = lr * max(1.0, shape[-2] / shape[-1]) ** 0.5
+    want = p0.double() * (1 - lr * decay) - alpha * o
+    off, size = float((p.double() - want).norm()), float(p0.double().norm() + alpha * o.norm())
+    assert off <= STATED * alpha * float(o.norm()) + 4 * 2.0 ** -24 * size
+    assert not torch.equal(p, p0)
