@@ -707,7 +707,7 @@ int blitz_quant_rows_write(const void* values, int value_type, int64_t value_str
   q.seed_ptr = seed_ptr;
   if (int rc = quant_sizes(q, kind, rows, n, N, D, group, "blitz_quant_rows_write: bad sizes, type or kind")) return rc;
   if (value_stride < D) return fail(BLITZ_EINVAL, "blitz_quant_rows_write: value_stride smaller than D");
-  if (n == 0 || D == 0) return 0;
+  if (n == 0 || D == 0 || N == 0) return 0;
   if (!values || !codes || !scales) return fail(BLITZ_EINVAL, "blitz_quant_rows_write: null pointer");
   return check(launch_quant_write(q, S(stream)), "blitz_quant_rows_write");
 }
@@ -735,7 +735,7 @@ int blitz_adam8_update(float* param, const float* grad, void* m_codes, float* m_
     return fail(BLITZ_EINVAL, "blitz_adam8_update: give either visible or rows");
   Adam8Params a{};
   a.n = rows ? n_rows : N;
-  if (a.n == 0) return 0;
+  if (a.n == 0 || N == 0) return 0;
   if (!param || !grad || !m_codes || !m_scales || !r_codes || !r_scales)
     return fail(BLITZ_EINVAL, "blitz_adam8_update: null pointer");
   a.param = param;

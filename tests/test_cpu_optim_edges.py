@@ -118,3 +118,10 @@ def test_groups_of_a_state_saved_without_their_size_are_the_optimizers(fake_kern
     q.grad = torch.ones(6, 100)
     _stepped(opt, p, torch.ones(1, 6, 100))
     assert opt.state[p]["exp_avg_scales"].shape == opt.state[q]["exp_avg_scales"].shape == (6, 4)
+
+
+def test_every_row_of_a_list_lies_outside_an_empty_store():
+    """And is skipped, as documented: an empty tensor has no address, and needs none."""
+    step = [1.0, 0.1, 0.9, 0.1, 0.999, 0.001, 1e-15]
+    assert _lib.call("blitz_quant_rows_write", 16, 0, 45, None, None, 1, 16, 3, 0, 45, 45, 0, 0, None, None) == 0
+    assert _lib.call("blitz_adam8_update", None, 16, *[None] * 4, None, 16, 3, *step, 0, 45, 45, 0, None, None) == 0

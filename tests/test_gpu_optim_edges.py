@@ -78,3 +78,13 @@ def test_an_update_in_a_part_of_the_gpu_equals_one_on_the_whole(cuda_device, sha
         part.pop_context()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert all(torch.equal(a, b) for a, b in zip(update(), want))
+
+
+def test_rows_of_an_empty_store(cuda_device):
+    codes = torch.zeros((0, 45), dtype=torch.uint8, device=cuda_device).view(torch.float8_e4m3fn)
+    scales, rows = torch.zeros((0, 1), device=cuda_device), torch.tensor([0, 5, -1], device=cuda_device)
+    x = torch.ones(3, 45, device=cuda_device)
+    ops.quant_rows_write(x, codes, scales, rows, group=45)
+    assert (ops.quant_rows_read(codes, scales, rows, group=45) == 0).all()
+    ops.adam8_update_rows(torch.zeros(0, 45, device=cuda_device), x, codes, scales, codes.clone(), scales.clone(), rows,
+                          0.1, 0.9, 0.999, 1e-15, 0, 45, group=45, seed=1)
