@@ -7,10 +7,10 @@
 // one thread, each followed by all warps turning the accumulators into f16
 // terms; no launch, no grid-wide barrier and no traffic beyond shared memory.  Bound by the
 // latency of that chain: what a block cannot overlap, the other blocks of
-// the SM do (small matrices: up to eight a SM).
+// the SM do (three at most: every matrix has tiles of 128 rows, 66 KB at least).
 //
-// One of 128 x 256 in 32 bits takes 53 us, 9 us a step: about 8k cycles of products and 7k of
-// conversions; 1000 of 64 x 64 take 102 us.
+// One of 128 x 256 in 32 bits takes 52 us, 9 us a step: about 8k cycles of products and 7k of
+// conversions; 1000 of 64 x 64 take 99 us.
 //
 // Within a product the small terms (high * low, low * high) come first: the
 // accumulator drops bits below its last one at every addition, so the sum

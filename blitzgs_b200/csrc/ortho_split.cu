@@ -10,7 +10,7 @@
 // block, so the result does not depend on timing.
 //
 // Where there are tiles enough (S = 1) a k of 64 takes 760 cycles, the products' own rate; 2048^2 in
-// 32 bits takes 480 us, 4096^2 3.9 ms.  (Tiles of 128 x 256 have fewer units in flight and leave
+// 32 bits takes 468 us, 4096^2 3.8 ms.  (Tiles of 128 x 256 have fewer units in flight and leave
 // more SMs without one: 4260 us for 3760 at 4096^2. Pairs of blocks on 256 x 128 took 5530.)
 //
 // The operands' ring holds the low terms of a k of 64 and the high ones as units of their own:

@@ -25,6 +25,9 @@ namespace quant {
 
 enum Kind : int { kInt8 = 0, kE4m3 = 1 };
 
+// The hash of (seed, row, column): odd multipliers between shifts.  0x9E3779B1 and 0x85EBCA77
+// are primes that Y. Collet published for hashing 32-bit words; 0x7FEB352D, 0x846CA68B and
+// 0x2C1B3C6D come from C. Wellons's published search for 32-bit mixers of little bias.
 __device__ __forceinline__ uint32_t row_key(uint32_t seed, int64_t row) {
   uint32_t k = seed * 0x9E3779B1u + (uint32_t)row * 0x85EBCA77u;
   k = (k ^ (k >> 16)) * 0x7FEB352Du;

@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(256) read_kernel(QuantParams p) {
 
 // V codes of one group by one thread, where rows and groups are whole numbers of
 // V and everything is aligned to it: one load and one or two stores for what
-// costs V of each above.  1M x 48 e4m3 -> bf16 (148 MB): 28 us, 81% of the measured copy rate, where
+// costs V of each above.  1M x 48 e4m3 -> bf16 (148 MB): 28.5 us, 79% of the measured copy rate, where
 // read_kernel takes 55.
 template <class T, int KIND, int V>
 __global__ void __launch_bounds__(256) read_vector_kernel(QuantParams p) {
@@ -158,8 +158,8 @@ __global__ void __launch_bounds__(256) read_vector_kernel(QuantParams p) {
   }
 }
 
-// 320k of 8M rows of 45: 113 us for 411 MB (scattered rows open whole sectors), against 36 us for
-// the 238 MB that the rows hold; issue slots 60% busy.  4 or 16 lanes a row took 137 and 131.
+// 320k of 8M rows of 45: 114 us for 411 MB (scattered rows open whole sectors), against 36 us for
+// the 238 MB that the rows hold; issue slots 59% busy.  4 or 16 lanes a row took 137 and 131.
 // One group of one row's step.  The moment updates are single rounded operations in
 // the order of the formula (no contraction), so the codes do not depend on how the
 // compiler fuses them.

@@ -131,9 +131,9 @@ __device__ __forceinline__ uint32_t smem_desc(uint32_t addr, uint32_t leading) {
   return ((addr >> 4) & 0x3fff) | (leading >> 4) << 16;
 }
 constexpr uint32_t kDescUpper = (1024u >> 4) | 1u << 14 | 2u << 29;
-// f16 x f16 -> f32; b_mn: B lies in memory with n contiguous
-__device__ __forceinline__ uint32_t instruction_desc(int bn, bool b_mn, uint32_t rows = 128) {
-  return 1u << 4 | (b_mn ? 1u << 16 : 0u) | (uint32_t)(bn >> 3) << 17 | (rows >> 4) << 24;
+// f16 x f16 -> f32, 128 rows; b_mn: B lies in memory with n contiguous
+__device__ __forceinline__ uint32_t instruction_desc(int bn, bool b_mn) {
+  return 1u << 4 | (b_mn ? 1u << 16 : 0u) | (uint32_t)(bn >> 3) << 17 | (128u >> 4) << 24;
 }
 // One product and one commit (and, above, copies).  The whole warp calls these with the
 // same operands and the lane that has `on` issues: where a branch picks the lane instead, the

@@ -1102,6 +1102,8 @@ def adam8_update_rows(param, grad_rows, m_codes, m_scales, r_codes, r_scales, ro
            group, seed, grad_scale, "adam8_update_rows")
 
 
+# the triple that K. Jordan published with momentum orthogonalised so (2024): the steepest at 0 that
+# still settles singular values around 1
 ORTHO_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 

@@ -99,8 +99,8 @@ class SparseGaussianAdam8bit(SparseGaussianAdam):
     change by less than half a step of 8 bits at a time.
 
     Rows of fewer than 8 values keep 32-bit moments: a scale of 4 bytes a row
-    would take back what the codes save.  A non-finite gradient makes the moments of its
-    whole group NaN (one scale holds them)."""
+    would take back what the codes save.  A gradient that is not finite, or whose square
+    is not, makes the moments of its whole group NaN (one scale holds them)."""
 
     _CODES = ("exp_avg_codes", "exp_root_codes")
 
