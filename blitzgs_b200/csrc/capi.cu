@@ -68,7 +68,7 @@ int ortho_fields(OrthoParams& p, const char* name, int type, int64_t batch, int6
   char text[160];
   snprintf(text, sizeof(text), "%s: bad sizes, type or steps", name);
   if (batch < 0 || rows < 0 || cols < 0 || rows > most || cols > most || type < 0 || type > 2 || steps < 1 ||
-      steps > 64 || !(eps >= 0.0f))
+      steps > kMostSteps || !(eps >= 0.0f))
     return fail(BLITZ_EINVAL, text);
   if (!ortho_coefficients_ok(a, b, c, steps)) {
     char text[160];

@@ -15,7 +15,8 @@
 // bf16 terms would need three for that.  16-bit inputs are exact in one term, so step 0
 // reads one of X; every other operand has two, whatever type the result is rounded to.
 // Everything is scaled by powers of two into
-// f16's range: |X_ij| <= 1.9 by 2^14 (by more where X is tiny throughout, see OrthoInfo), |A_ij| <= 3.7 by 2^14, |B_ij| < 7.9 by 2^13
+// f16's range: |X_ij| <= 1.9 by 2^14 (by more where X is tiny throughout, see OrthoInfo),
+// |A_ij| <= 3.7 by 2^14, |B_ij| < 7.9 by 2^13
 // (the caller's coefficients are checked to keep to that).
 //
 // Which kernel runs goes by size: registers or one block's shared memory (ortho_small.cu), one
@@ -29,7 +30,7 @@
 // Every wait gives up after two seconds (see wait_limit).  In `resident_kernel` that block's matrix
 // is then NaN.  Over the grid the other blocks learn of it at the next barrier, and
 // `lost_kernel`, which runs when all of them have ended and so after all that they wrote, makes all
-// outputs of the call NaN.  (In a call of 127 us its launch does not show.)
+// outputs of the call NaN.  (In a call of 124 us its launch does not show.)
 #include <algorithm>
 
 #include "ortho_grid.cuh"
@@ -120,9 +121,8 @@ __global__ void __launch_bounds__(256) layout_kernel(LayoutParams p) {
 #pragma unroll
     for (int k = 16; k > 0; k >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, k);
     if (tid == 0) {
-      const OrthoInfo info = ortho_scaling(sqrt(sq), o);
-      up_shared = info.up;
-      if (r == 0) p.info[b] = info;
+      up_shared = ortho_up(sqrt(sq));
+      if (r == 0) ortho_scaling(sqrt(sq), o, p.info + b);
     }
   }
   if (!wide) {

@@ -11,35 +11,66 @@ namespace blitz {
 // the powers of two that X (at least, see OrthoInfo), A and B are scaled by in f16 terms (see ortho.cu)
 constexpr float kScaleX = 16384.0f, kScaleA = 16384.0f, kScaleB = 8192.0f;
 
-// How one matrix is scaled into f16.  u with 2-norm `norm` is stored as u * up.x * up.y, exactly
-// (two factors, since 2^163 is no float), with norm times that in [2^13, 2^14).  X_1 and what
-// follows are stored times x = 2^14 2^k, with k > 0 where u is so much smaller than eps that the
-// iterates stay small: they would lie among f16's denormals (in 40 x 60 with eps = 1e-7, 1.6e-3 off
-// for a norm of 1e-15).  X_0 times x is `first` times what is stored of u; inv is 1 / x.
+// How one matrix is scaled into f16.  u is stored as u * up.x * up.y (ortho_up).  X_i, i > 0,
+// is stored times 2^(14 + k[i]), with k[i] > 0 where u is so much smaller than eps (or the
+// coefficients so small) that this iterate is small: it would lie among f16's denormals (40 x 60
+// with eps = 1e-7 came out 1.6e-3 off for a norm of 1e-15).  X_1 so scaled is B_0 times
+// `first` times what is stored of u.
 struct OrthoInfo {
   float2 up;
-  float first, inv;
+  float first;
+  uint8_t k[kMostSteps + 4];
 };
-__device__ __forceinline__ OrthoInfo ortho_scaling(double norm, const OrthoParams& p) {
-  OrthoInfo info;
-  const int e = max(-126, norm > 0.0 && norm <= 1e300 ? 14 - (ilogb(norm) + 1) : 0);
-  info.up = make_float2(ldexpf(1.0f, min(e, 80)), ldexpf(1.0f, max(e - 80, 0)));
-  int k = 0;
-  if (norm < (double)p.eps) {
+
+__device__ __forceinline__ float ortho_pow2(int e) { return __int_as_float((127 + e) << 23); }
+
+// the exponent that takes a 2-norm into [2^13, 2^14) (less for the largest, whose values are then
+// still below 4)
+__device__ __forceinline__ int ortho_exponent(double norm) {
+  return max(-126, norm > 0.0 && norm <= 1e300 ? 14 - (ilogb(norm) + 1) : 0);
+}
+// exact, in two factors, since 2^163 is no float
+__device__ __forceinline__ float2 ortho_up(double norm) {
+  const int e = ortho_exponent(norm);
+  return make_float2(ortho_pow2(min(e, 80)), ortho_pow2(max(e - 80, 0)));
+}
+__device__ __forceinline__ void ortho_scaling(double norm, const OrthoParams& p, OrthoInfo* info) {
+  info->up = ortho_up(norm);
+  const double a = fabs((double)p.a), b = fabs((double)p.b), c = fabs((double)p.c);
+  int first = 0;
+  if (norm < (double)p.eps || a + b + c < 1.0) {
     // bounds of the iterates: a step multiplies singular values up to s by at most
-    // |a| + |b| s^2 + |c| s^4, and they stay below 1.85 (checked by the caller)
-    double s = norm / (norm + (double)p.eps), most = s;
-    for (int i = 0; i < p.steps; ++i) {
-      const double l = s * s;
-      s = fmin(s * (fabs((double)p.a) + l * (fabs((double)p.b) + l * fabs((double)p.c))), 1.85);
-      most = fmax(most, s);
+    // a + b s^2 + c s^4, and they stay below 1.85 (checked by the caller)
+    double s = norm / (norm + (double)p.eps);
+    for (int i = 0; i <= p.steps; ++i) {
+      const int k = s > 0.0 ? max(0, min(100, ilogb(1.85 / s))) : 0;
+      info->k[i] = (uint8_t)k;
+      if (i == 1) first = k;
+      s = fmin(s * (a + s * s * (b + s * s * c)), 1.85);
     }
-    if (most > 0.0) k = max(0, min(100, ilogb(1.85 / most)));
+  } else {
+    for (int i = 0; i <= p.steps; ++i) info->k[i] = 0;
   }
-  info.inv = ldexpf(1.0f / kScaleX, -k);
   // zeros stay zeros, whatever eps is
-  info.first = norm == 0.0 ? 0.0f : (float)(1.0 / ((norm + (double)p.eps) * ldexp((double)info.inv, e)));
-  return info;
+  info->first = norm == 0.0 ? 0.0f
+                            : (float)(1.0 / ((norm + (double)p.eps) * ldexp(1.0, ortho_exponent(norm) - 14 - first)));
+}
+// what a step's sums are multiplied by: those of X X^T squared, to give A; those of B X, to give the
+// next X as it is stored, or the direction
+struct OrthoFactors {
+  float x, next;
+};
+__device__ __forceinline__ OrthoFactors ortho_factors(const OrthoInfo& info, int step, bool last) {
+  const int k = info.k[step], to = info.k[step + 1];
+  OrthoFactors f;
+  if (step == 0) {
+    f.x = info.first * ortho_pow2(-14 - to);
+    f.next = (last ? f.x : info.first) / kScaleB;
+  } else {
+    f.x = ortho_pow2(-14 - k);
+    f.next = (last ? f.x : ortho_pow2(to - k)) / kScaleB;
+  }
+  return f;
 }
 
 // whether u needs two f16 terms

@@ -24,6 +24,8 @@ struct OrthoParams {
   long long wait_limit;  // cycles after which a wait within a kernel gives up
 };
 
+constexpr int kMostSteps = 64;
+
 // about two seconds of the SM's clock
 constexpr long long kOrthoWaitLimit = 4000000000ll;
 

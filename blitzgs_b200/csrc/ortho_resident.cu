@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) resident_kernel(OrthoP
       __syncthreads();
       if (tid == 0) {
         for (int w = 1; w < THREADS / 32; ++w) sq += sums[w];
-        scaling = ortho_scaling(sqrt(sq), p);
+        ortho_scaling(sqrt(sq), p, &scaling);
       }
       __syncthreads();
       const float2 up = scaling.up;
@@ -194,13 +194,12 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) resident_kernel(OrthoP
     }
     fence_async_shared();
     __syncthreads();
-    const float first = scaling.first, inv = scaling.inv;
 
 #pragma unroll 1
     for (int s = 0; s < p.steps; ++s) {
       const bool two_x = s > 0 || two_in;
       const bool last = s + 1 == p.steps;
-      const float from = s == 0 ? first : 1.0f, fx = from * inv;
+      const OrthoFactors by = ortho_factors(scaling, s, last);
 #pragma unroll 1
       for (int which = 0; which < 3; ++which) {
         if (warp == 0) {
@@ -228,7 +227,7 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) resident_kernel(OrthoP
           tmem_load32(tmem_rows + c, v);
           if (which == 2 && last) {
             // the direction in 32 bits over X, in the order of the matrix's own memory
-            const float f = fx / kScaleB;
+            const float f = by.next;
             if (row < n) {
               if (wide) {
                 float* dst = (float*)X + row * stage_stride(m) + c;
@@ -246,8 +245,8 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) resident_kernel(OrthoP
           // columns past np / mp hold what was left there; nothing reads their terms
           uint8_t* dst = which == 2 ? X : A;
           const int term = which == 2 ? l.x_term : l.a_term;
-          const float f = which == 0 ? fx * fx * kScaleA : which == 1 ? p.c * (kScaleB / (kScaleA * kScaleA))
-                                                                     : from / kScaleB;
+          const float f = which == 0 ? by.x * by.x * kScaleA : which == 1 ? p.c * (kScaleB / (kScaleA * kScaleA))
+                                                                     : by.next;
           const float fb = p.b * (kScaleB / kScaleA);
 #pragma unroll
           for (int k = 0; k < 32; k += 8) {

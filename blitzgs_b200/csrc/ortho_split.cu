@@ -20,7 +20,8 @@
 // 100; one warp each took 1350 cycles a k of 64.
 //
 // Tensor memory holds four accumulators. Each takes one k of 64 (the low terms first) and
-// is then added up in registers: the tensor cores' additions drop the bits below the accumulator's last one, those here round. Over
+// is then added up in registers: the tensor cores' additions drop the bits below the
+// accumulator's last one, those here round. Over
 // 1024 columns that is the difference between an error of 4e-5 and of 2e-6.
 #include <algorithm>
 #include <atomic>
@@ -121,13 +122,11 @@ __device__ __forceinline__ void store_terms(__half* dst, int64_t low, int left, 
 template <int C>
 __device__ __forceinline__ void finish(const OrthoGrid& p, const OrthoTerms& t, int b, int row, int col, bool diagonal,
                                        bool mirror, float (&v)[C], const uint32_t (&old_hi)[C / 2],
-                                       const uint32_t (&old_lo)[C / 2], float first, float inv) {
+                                       const uint32_t (&old_lo)[C / 2], OrthoFactors by) {
   const int n = (int)p.o.n, m = (int)p.o.m, lane = threadIdx.x & 31;
-  const float from = t.step == 0 ? first : 1.0f;
   if (t.which == kApply) {
-    const float f = (t.last ? from * inv : from) / kScaleB;
 #pragma unroll
-    for (int k = 0; k < C; ++k) v[k] *= f;
+    for (int k = 0; k < C; ++k) v[k] *= by.next;
     if (row >= n) return;
     if (!t.last) {
       uint32_t h[C / 2], l[C / 2];
@@ -180,7 +179,7 @@ __device__ __forceinline__ void finish(const OrthoGrid& p, const OrthoTerms& t, 
   }
   const int64_t low = (int64_t)n * p.ldn;
   if (t.which == kGram) {
-    const float fx = from * inv, f = fx * fx * kScaleA;
+    const float f = by.x * by.x * kScaleA;
 #pragma unroll
     for (int k = 0; k < C; ++k) v[k] *= f;
   } else {
@@ -369,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
         tile_of(s, t, b, mi, ni);
         const int row = mi * kB + local, col = ni * kB + (S > 1 ? rank * W : 0) + half * C;
         // read ahead of the sums
-        const float first_x = p.info[b].first, inv_x = p.info[b].inv;
+        const OrthoFactors factors = ortho_factors(p.info[b], s.t.step, s.t.last);
         const bool sym = s.t.which != kApply, diagonal = sym && mi == ni, mirror = sym && mi > ni;
         float acc[64];
 #pragma unroll
@@ -407,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = acc[c + i];
             load_a<32>(p, s.t, b, row, col + c, hi, lo);
-            finish<32>(p, s.t, b, row, col + c, diagonal, mirror, v, hi, lo, first_x, inv_x);
+            finish<32>(p, s.t, b, row, col + c, diagonal, mirror, v, hi, lo, factors);
           }
         } else {
           // slots of W / 4 columns x 128 rows of 4 columns' sums; one for each other block, in
@@ -470,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const __grid_constan
           }
           __syncwarp();
           if (lane < S && lane != rank && ok) peer_arrive(peer_addr(x_empty, lane));
-          finish<C>(p, s.t, b, row, col, diagonal, mirror, sum, old_hi, old_lo, first_x, inv_x);
+          finish<C>(p, s.t, b, row, col, diagonal, mirror, sum, old_hi, old_lo, factors);
         }
       }
     }

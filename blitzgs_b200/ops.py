@@ -1126,7 +1126,7 @@ def orthogonalize(g, *, steps=5, coefficients=ORTHO_COEFFICIENTS, eps=1e-7):
     """The direction of each matrix of g [..., rows, cols] (float32, bfloat16
     or float16): its singular values driven towards 1 by ``steps`` Newton-Schulz
     steps (blitz_orthogonalize).  Returns a new tensor of g's type, within
-    about 1e-5 (2-norm) of the formula before its rounding to that type.  Not
+    about 1e-5 (2-norm, five steps) of the formula before its rounding to that type.  Not
     differentiable: where gradients are on, a g that requires one is refused."""
     _no_graph(g, "orthogonalize")
     _same_device(g)

@@ -66,6 +66,21 @@ def test_updates_far_smaller_than_eps(cuda_device, shape):
             assert beyond_rounding(got, formula(g, steps=steps)) <= 1e-5, (norm, steps)
 
 
+@pytest.mark.parametrize("shape", [(9, 14), (24, 40), (100, 250), (200, 150), (150, 160)])
+def test_many_steps_from_far_below_eps(cuda_device, shape):
+    """Iterates that are small at first and not at last, and ones that shrink.  (1.875 is the largest
+    factor of the convergent triple; every step is one of the same kind, and the roundings of early
+    ones, 2^-22 each, are multiplied no more than the iterates themselves: the sum of 30 stays below
+    30 * 4 * 2^-22 = 2.9e-5 of the result.)"""
+    base = matrices(shape, torch.float32, "cpu")
+    convergent, halving = (1.875, -1.25, 0.375), (0.5, 0.0, 0.0)
+    for norm, steps, co in ((1e-12, 25, convergent), (1e-14, 30, convergent), (1e-17, 25, convergent),
+                            (1e-25, 64, convergent), (1e-3, 30, halving), (1e-12, 30, halving)):
+        g = (base * (norm / base.norm())).to(cuda_device)
+        got, want = ops.orthogonalize(g, steps=steps, coefficients=co), formula(g, steps=steps, coefficients=co)
+        assert float((got.double() - want).norm() / want.norm()) <= 30 * 4 * 2.0 ** -22, (norm, steps, co)
+
+
 @pytest.mark.parametrize("shape", [(1, 3), (12, 3), (9, 14), (24, 40), (100, 250), (200, 150), (150, 160)])
 def test_the_smallest_and_largest_updates_without_eps(cuda_device, shape):
     """The direction of what 32 bits hold, down to numbers that are denormal themselves."""
