@@ -729,7 +729,8 @@ int blitz_adam8_update(float* param, const float* grad, void* m_codes, float* m_
                        float* r_scales, const uint8_t* visible, const int64_t* rows, int64_t n_rows, float grad_scale,
                        float lr, float b1, float one_minus_b1, float b2, float one_minus_b2, float eps, int64_t N,
                        int64_t M, int group, uint32_t seed, const int64_t* seed_ptr, void* stream) {
-  if (N < 0 || M <= 0 || M > kMaxRow || n_rows < 0 || group < 1 || group > 256 || too_many_units(rows ? n_rows : N, M, group))
+  if (N < 0 || M <= 0 || M > kMaxRow || n_rows < 0 || group < 1 || group > 256 ||
+      too_many_units(rows ? n_rows : N, M, group))
     return fail(BLITZ_EINVAL, "blitz_adam8_update: bad sizes");
   if ((visible != nullptr) == (rows != nullptr) && (rows || N > 0))
     return fail(BLITZ_EINVAL, "blitz_adam8_update: give either visible or rows");

@@ -588,8 +588,8 @@ int blitz_adam8_update(float* param, const float* grad, void* m_codes, float* m_
  * time need their own.
  */
 /* How many cycles of the SM's clock a wait within these kernels lasts before it
- * gives up, which makes all outputs (the parameter; not the momentum) of the call NaN, or, for matrices
- * that one block holds, of that block's matrices; sets it for the calls that follow (negative: no change) and
+ * gives up.  All outputs of the call are then NaN (the parameter; the momentum
+ * is right), or, for matrices that one block holds, that block's.  Sets it for the calls that follow (negative: no change) and
  * returns what it was, at first 4e9 (about two seconds). */
 int64_t blitz_orthogonalize_wait_limit(int64_t cycles);
 size_t blitz_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols);
